@@ -1526,6 +1526,183 @@ int pdattn_append_kv(const void* k_new, const void* v_new, void* k_cache, void* 
     return PDATTN_OK;
 }
 
+int pdattn_rope_frequencies(int rotary_dim, double base, int scaling, double factor, double trained_len,
+                            double slow, double fast, double* h_freq, float* attn_scale) {
+    if (!h_freq || !attn_scale) return fail(PDATTN_ERR_INVALID_ARGUMENT, "null output");
+    if (rotary_dim < 2 || rotary_dim > kHeadDim || rotary_dim % 2)
+        return fail(PDATTN_ERR_INVALID_ARGUMENT, "rotary_dim=%d must be even, in [2, %d]", rotary_dim, kHeadDim);
+    if (scaling < PDATTN_ROPE_PLAIN || scaling > PDATTN_ROPE_WAVELENGTH)
+        return fail(PDATTN_ERR_INVALID_ARGUMENT, "unknown scaling %d", scaling);
+    if (!std::isfinite(base) || base <= 1.0 || !std::isfinite(factor) || factor < 1.0)
+        return fail(PDATTN_ERR_INVALID_ARGUMENT, "base must be above 1 and factor at least 1");
+    const bool ramp = scaling == PDATTN_ROPE_YARN || scaling == PDATTN_ROPE_WAVELENGTH;
+    if (ramp && !(std::isfinite(trained_len) && trained_len > 0 && slow > 0 && fast > slow && std::isfinite(fast)))
+        return fail(PDATTN_ERR_INVALID_ARGUMENT, "trained_len must be positive, and 0 < slow < fast");
+    constexpr double kTwoPi = 6.283185307179586;
+    if (scaling == PDATTN_ROPE_BASE && rotary_dim > 2) base *= std::pow(factor, rotary_dim / (rotary_dim - 2.0));
+    // the pair index at which a frequency turns `turns` times in trained_len positions
+    auto pair_of = [&](double turns) { return rotary_dim * std::log(trained_len / (turns * kTwoPi)) / (2 * std::log(base)); };
+    const double lo = ramp ? std::max(std::floor(pair_of(fast)), 0.0) : 0.0;
+    const double hi = ramp ? std::min(std::ceil(pair_of(slow)), rotary_dim - 1.0) : 0.0;
+    for (int i = 0; i < rotary_dim / 2; ++i) {
+        double f = std::pow(base, -2.0 * i / rotary_dim), keep = 1.0;
+        if (scaling == PDATTN_ROPE_LINEAR) keep = 0.0;
+        if (scaling == PDATTN_ROPE_YARN) keep = 1.0 - std::min(1.0, std::max(0.0, (i - lo) / std::max(hi - lo, 1e-3)));
+        if (scaling == PDATTN_ROPE_WAVELENGTH)
+            keep = std::min(1.0, std::max(0.0, (trained_len * f / kTwoPi - slow) / (fast - slow)));
+        h_freq[i] = f / factor * (1.0 - keep) + f * keep;
+    }
+    *attn_scale = scaling == PDATTN_ROPE_YARN ? (float)(0.1 * std::log(factor) + 1.0) : 1.0f;
+    return PDATTN_OK;
+}
+
+int pdattn_rope_append_kv(const pdattn_rope_append_params* p, void* stream) {
+    if (!p) return fail(PDATTN_ERR_INVALID_ARGUMENT, "null params");
+    if (p->n < 0 || p->B < 0 || p->Hkv <= 0 || p->Hq < 0 || p->Hq > 4096 || p->Hkv > 4096)
+        return fail(PDATTN_ERR_INVALID_ARGUMENT, "n=%d B=%d Hq=%d Hkv=%d", p->n, p->B, p->Hq, p->Hkv);
+    if (p->rotary_dim < 2 || p->rotary_dim > kHeadDim || p->rotary_dim % 2)
+        return fail(PDATTN_ERR_INVALID_ARGUMENT, "rotary_dim=%d must be even, in [2, %d]", p->rotary_dim, kHeadDim);
+    if (!std::isfinite(p->scale)) return fail(PDATTN_ERR_INVALID_ARGUMENT, "scale is not finite");
+    if ((p->q == nullptr) != (p->Hq == 0)) return fail(PDATTN_ERR_INVALID_ARGUMENT, "q is NULL just when Hq is 0");
+    if (p->n == 0) return PDATTN_OK;
+    if (!p->k_new || !p->v_new || !p->k_cache || !p->v_cache || !p->kv_indptr || !p->kv_indices || !p->batch_idx ||
+        !p->positions || !p->freq || (p->q && !p->q_out))
+        return fail(PDATTN_ERR_INVALID_ARGUMENT, "null device pointer");
+    for (const void* x : {p->q, p->k_new, p->v_new, static_cast<const void*>(p->q_out), static_cast<const void*>(p->k_cache),
+                          static_cast<const void*>(p->v_cache)})
+        if (!aligned16(x)) return fail(PDATTN_ERR_INVALID_ARGUMENT, "q, K/V, q_out and caches must be 16-byte aligned");
+    if (p->n > 1) {
+        const int64_t qw = (int64_t)p->Hq * kHeadDim, kw = (int64_t)p->Hkv * kHeadDim;
+        if ((p->q && (p->q_stride % 8 || p->q_stride < qw)) || p->k_stride % 8 || p->k_stride < kw || p->v_stride % 8 ||
+            p->v_stride < kw)
+            return fail(PDATTN_ERR_INVALID_ARGUMENT, "token strides must be multiples of 8 elements that hold a token's heads");
+        if (p->q && p->q_out == p->q && p->q_stride != qw)
+            return fail(PDATTN_ERR_INVALID_ARGUMENT, "q_out is contiguous: q can be rotated in place only if it is");
+    }
+    DeviceFacts f;
+    if (int st = device_facts(&f)) return st;
+    RopeArgs a;
+    a.q = p->q;
+    a.k_new = p->k_new;
+    a.v_new = p->v_new;
+    a.q_out = p->q_out;
+    a.k_cache = p->k_cache;
+    a.v_cache = p->v_cache;
+    a.kv_indptr = p->kv_indptr;
+    a.kv_indices = p->kv_indices;
+    a.batch_idx = p->batch_idx;
+    a.positions = p->positions;
+    a.rope_positions = p->rope_positions;
+    a.freq = p->freq;
+    a.n_invalid = p->n_invalid;
+    a.q_stride = p->q_stride * 2;
+    a.k_stride = p->k_stride * 2;
+    a.v_stride = p->v_stride * 2;
+    a.n = p->n;
+    a.B = p->B;
+    a.Hq = p->Hq;
+    a.Hkv = p->Hkv;
+    a.rotary_dim = p->rotary_dim;
+    a.interleaved = p->interleaved != 0;
+    a.scale = p->scale;
+    if (p->q) res_written(p->q_out, (size_t)p->n * p->Hq * kHeadDim * 2);
+    PD_HIP(launch_rope_append(a, f.cus, static_cast<hipStream_t>(stream)));
+    return PDATTN_OK;
+}
+
+}  // extern "C"
+
+namespace {
+
+int check_tree_params(const pdattn_tree_params* p, int* G) {
+    if (!p) return fail(PDATTN_ERR_INVALID_ARGUMENT, "null params");
+    if (p->B < 0 || p->n_tokens < 0) return fail(PDATTN_ERR_INVALID_ARGUMENT, "B=%d n_tokens=%d", p->B, p->n_tokens);
+    if (int st = check_heads(p->Hq, p->Hkv, G)) return st;
+    if ((int64_t)p->n_tokens * p->Hq > (1 << 30)) return fail(PDATTN_ERR_INVALID_ARGUMENT, "too many rows");
+    if (!p->q_indptr && p->n_tokens != p->B)
+        return fail(PDATTN_ERR_INVALID_ARGUMENT, "without q_indptr there is one token per sequence: n_tokens=%d B=%d", p->n_tokens, p->B);
+    if (p->max_tokens < 1) return fail(PDATTN_ERR_INVALID_ARGUMENT, "max_tokens=%d must be >= 1", p->max_tokens);
+    if ((p->mask || p->depth) && p->max_tokens > PDATTN_TREE_MAX_TOKENS)
+        return fail(PDATTN_ERR_UNSUPPORTED, "max_tokens=%d > %d with a mask or depths", p->max_tokens, PDATTN_TREE_MAX_TOKENS);
+    if (p->mask && p->mask_words < 1) return fail(PDATTN_ERR_INVALID_ARGUMENT, "mask_words=%d must be >= 1", p->mask_words);
+    if (!std::isfinite(p->sm_scale)) return fail(PDATTN_ERR_INVALID_ARGUMENT, "sm_scale is not finite");
+    const pdattn_score_params& sc = p->score;
+    if (!std::isfinite(sc.soft_cap) || sc.soft_cap < 0.f)
+        return fail(PDATTN_ERR_INVALID_ARGUMENT, "soft_cap must be finite and not negative");
+    if (sc.window < 0 || sc.sink < 0) return fail(PDATTN_ERR_INVALID_ARGUMENT, "window=%d sink=%d", sc.window, sc.sink);
+    if (p->B == 0 || p->n_tokens == 0) return PDATTN_OK;
+    if (!p->q || !p->k_cache || !p->v_cache || !p->kv_indptr || !p->kv_indices || !p->kv_last_page_len)
+        return fail(PDATTN_ERR_INVALID_ARGUMENT, "null device pointer in params");
+    if (!aligned16(p->q) || !aligned16(p->k_cache) || !aligned16(p->v_cache))
+        return fail(PDATTN_ERR_INVALID_ARGUMENT, "q / k_cache / v_cache must be 16-byte aligned");
+    return PDATTN_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t pdattn_tree_workspace_size(const pdattn_tree_params* p) {
+    int G = 0;
+    if (check_tree_params(p, &G) != PDATTN_OK || p->B == 0 || p->n_tokens == 0) return 0;
+    return kAlign;
+}
+
+int pdattn_tree_attention(const pdattn_tree_params* p, void* out, float* lse, pdattn_workspace* ws,
+                          void* stream) {
+    int G = 0;
+    if (int st = check_tree_params(p, &G)) return st;
+    if (p->B == 0 || p->n_tokens == 0) return PDATTN_OK;
+    if (!out || !lse) return fail(PDATTN_ERR_INVALID_ARGUMENT, "null out / lse");
+    if (!aligned16(out)) return fail(PDATTN_ERR_INVALID_ARGUMENT, "out must be 16-byte aligned");
+    const size_t need = pdattn_tree_workspace_size(p);
+    if (int st = ensure_ws(ws, need)) return st;
+    res_written(ws->base, need);
+    res_written_outputs(out, lse, (size_t)p->n_tokens * p->Hq);
+    TreeArgs a;
+    a.q = static_cast<const _Float16*>(p->q);
+    a.k = static_cast<const uint8_t*>(p->k_cache);
+    a.v = static_cast<const uint8_t*>(p->v_cache);
+    a.kv_indptr = p->kv_indptr;
+    a.kv_indices = p->kv_indices;
+    a.kv_last = p->kv_last_page_len;
+    a.q_indptr = p->q_indptr;
+    a.mask = p->mask;
+    a.depth = p->depth;
+    a.slopes = p->score.slopes;
+    a.out = static_cast<_Float16*>(out);
+    a.lse = lse;
+    a.B = p->B;
+    a.Hq = p->Hq;
+    a.Hkv = p->Hkv;
+    a.G = G;
+    a.n_tokens = p->n_tokens;
+    a.mask_words = p->mask_words;
+    a.window = p->score.window;
+    a.sink = p->score.sink;
+    a.scale_log2 = p->sm_scale * 1.4426950408889634f;
+    a.cap_in = p->score.soft_cap > 0.f ? p->sm_scale / p->score.soft_cap : 0.f;
+    a.cap_out = p->score.soft_cap * 1.4426950408889634f;
+    PD_HIP(launch_tree_attention(a, static_cast<hipStream_t>(stream)));
+    return PDATTN_OK;
+}
+
+int pdattn_accept_kv(void* k_cache, void* v_cache, const int32_t* kv_indptr, const int32_t* kv_indices,
+                     const int32_t* kv_last_page_len, const int32_t* q_indptr,
+                     const int32_t* accepted_indptr, const int32_t* accepted, int B, int Hkv,
+                     int32_t* n_invalid, void* stream) {
+    if (B < 0 || Hkv <= 0 || Hkv > 4096) return fail(PDATTN_ERR_INVALID_ARGUMENT, "B=%d Hkv=%d", B, Hkv);
+    if (B == 0) return PDATTN_OK;
+    if (!k_cache || !v_cache || !kv_indptr || !kv_indices || !kv_last_page_len || !q_indptr || !accepted_indptr || !accepted)
+        return fail(PDATTN_ERR_INVALID_ARGUMENT, "null device pointer");
+    if (!aligned16(k_cache) || !aligned16(v_cache))
+        return fail(PDATTN_ERR_INVALID_ARGUMENT, "caches must be 16-byte aligned");
+    AcceptArgs a{k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len, q_indptr, accepted_indptr, accepted,
+                 n_invalid, B, Hkv};
+    PD_HIP(launch_accept_kv(a, static_cast<hipStream_t>(stream)));
+    return PDATTN_OK;
+}
+
 int pdattn_stream_read(const void* buf, size_t bytes, uint32_t* sink, void* stream) {
     if (!buf || !sink || bytes % 16) return fail(PDATTN_ERR_INVALID_ARGUMENT, "buf/sink null or bytes %% 16 != 0");
     if (bytes == 0) return PDATTN_OK;

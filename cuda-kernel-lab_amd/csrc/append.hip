@@ -1,5 +1,5 @@
-// append.hip -- paged KV append: the step before decode that writes new tokens' K/V into the
-// paged caches.
+// append.hip -- the write side of the paged caches: the append of new tokens' K/V (the step before decode),
+// the same with the rotary positions of q and k, and the move of accepted drafted tokens' rows.
 //
 // Layout of the caches and the page table as in the decode path (qilem/cuda-kernel-lab,
 // 01_decode_attention.cu:5-9, 112; FlashInfer's page-table convention): element (page, slot,
@@ -111,7 +111,201 @@ __global__ __launch_bounds__(kAppendThreads) void append_kv_kernel(AppendArgs a)
     }
 }
 
+// ---- rotary positions and the append in one pass -------------------------------------------------
+//
+// A token's rows (its Hq rows of q, Hkv of k, Hkv of v) are moved by 16 lanes each, 16 bytes per lane.
+// The pairs of a rotated row are (dim, dim + half), whose other halves lie in another lane of the row's
+// 16 (an exchange between lanes), or neighbours, both in the lane. cos and sin of a token's angles are
+// worked out once per workgroup, into LDS, while the rows' loads are on the way: the angle p f in 64
+// bits, reduced to a fraction of a turn there (p f may be 2^31 radians, of which 32 bits would leave no
+// fraction), then sin and cos of pi x in 32 bits. A row is read by one wave before any lane of it writes,
+// so q may be rotated in place.
+// Byte work, bound by HBM: every row is read once and written once.
+constexpr int kRopeThreads = 256;
+constexpr int kRopeRows = 4;          // rows of a 16-lane group on the way at once
+constexpr int kRopeMaxTokens = 8;     // tokens per workgroup
+constexpr int kRopeMaxPairs = kHeadDim / 2;
+
+typedef _Float16 rf16x8 __attribute__((ext_vector_type(8)));
+
+__global__ __launch_bounds__(kRopeThreads) void rope_append_kernel(RopeArgs a) {
+    __shared__ float2 s_cs[kRopeMaxTokens][kRopeMaxPairs];
+    __shared__ long long s_dst[kRopeMaxTokens];   // byte offset of the token's slot row in the caches, or -1
+    const int tid = threadIdx.x, lane = tid & 63, c = lane & 15;
+    const int R = a.Hq + 2 * a.Hkv, half = a.rotary_dim / 2;
+    const int t0 = blockIdx.x * a.tpb, ntok = min(a.tpb, a.n - t0), rows = ntok * R;
+
+    auto source = [&](int row, int& tok, int& r) {
+        tok = (int)div_by((uint32_t)row, (uint32_t)R, a.rows_m);
+        r = row - tok * R;
+        const int64_t t = t0 + tok;
+        const char* p = r < a.Hq ? static_cast<const char*>(a.q) + t * a.q_stride + r * 256
+                      : r < a.Hq + a.Hkv ? static_cast<const char*>(a.k_new) + t * a.k_stride + (r - a.Hq) * 256
+                                         : static_cast<const char*>(a.v_new) + t * a.v_stride + (r - a.Hq - a.Hkv) * 256;
+        return p;
+    };
+    u32x4 val[kRopeRows];
+    auto load = [&](int base) {
+#pragma unroll
+        for (int u = 0; u < kRopeRows; ++u) {
+            const int row = base + u * (kRopeThreads / 16);
+            int tok, r;
+            if (row < rows) val[u] = reinterpret_cast<const u32x4*>(source(row, tok, r))[c];
+        }
+    };
+    load(tid >> 4);
+
+    if (tid < ntok && a.Hkv > 0) {
+        const int t = t0 + tid, b = a.batch_idx[t], pos = a.positions[t];
+        const bool ok_b = b >= 0 && b < a.B;
+        const int pb = ok_b ? a.kv_indptr[b] : 0, np = ok_b ? a.kv_indptr[b + 1] - pb : 0;
+        long long dst = -1;
+        if (ok_b && pos >= 0 && pos / kPage < np) {
+            const size_t page = (size_t)(uint32_t)a.kv_indices[pb + pos / kPage];
+            dst = (long long)((page * kPage + pos % kPage) * a.Hkv * 256);
+        } else if (a.n_invalid) {
+            atomicAdd(a.n_invalid, 1);
+        }
+        s_dst[tid] = dst;
+    }
+    for (int i = tid; i < ntok * half; i += kRopeThreads) {
+        const int tok = i / half, pair = i - tok * half, t = t0 + tok;
+        const int pos = a.rope_positions ? a.rope_positions[t] : a.positions[t];
+        const double turns = (double)pos * a.freq[pair] * 0.15915494309189535;   // 1 / (2 pi)
+        float sn, cs;
+        sincospif(2.f * (float)(turns - rint(turns)), &sn, &cs);
+        s_cs[tok][pair] = make_float2(cs * a.scale, sn * a.scale);
+    }
+    __syncthreads();
+
+    for (int base = tid >> 4; base - (tid >> 4) < rows; base += kRopeRows * (kRopeThreads / 16)) {   // uniform
+        if (base != tid >> 4) load(base);
+#pragma unroll
+        for (int u = 0; u < kRopeRows; ++u) {
+            const int row = base + u * (kRopeThreads / 16);
+            const bool ok = row < rows;
+            int tok = 0, r = 0;
+            const char* src = ok ? source(row, tok, r) : nullptr;
+            const bool turn = ok && r < a.Hq + a.Hkv && 8 * c < a.rotary_dim;
+            rf16x8 x = __builtin_bit_cast(rf16x8, val[u]);
+            if (a.interleaved) {
+                if (turn) {
+#pragma unroll
+                    for (int e = 0; e < 8; e += 2) {
+                        if (8 * c + e >= a.rotary_dim) break;
+                        const float2 w = s_cs[tok][4 * c + e / 2];
+                        const float p = (float)x[e], n = (float)x[e + 1];
+                        x[e] = (_Float16)(p * w.x - n * w.y);
+                        x[e + 1] = (_Float16)(n * w.x + p * w.y);
+                    }
+                }
+            } else {
+                rf16x8 y;
+                if (half % 8 == 0) {   // (uniform) the pair's other half is a whole lane's piece
+                    const int other = (lane & 48) | ((8 * c < half ? c + half / 8 : c - half / 8) & 15);
+                    u32x4 o;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o[i] = (uint32_t)__shfl((int)val[u][i], other, 64);
+                    y = __builtin_bit_cast(rf16x8, o);
+                } else if (turn) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const int d = 8 * c + e, p = d < half ? d + half : d - half;
+                        y[e] = d < a.rotary_dim ? reinterpret_cast<const _Float16*>(src)[p] : (_Float16)0.f;
+                    }
+                }
+                if (turn) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const int d = 8 * c + e;
+                        if (d >= a.rotary_dim) break;
+                        const bool lo = d < half;
+                        const float2 w = s_cs[tok][lo ? d : d - half];
+                        x[e] = (_Float16)((float)x[e] * w.x + (float)y[e] * (lo ? -w.y : w.y));
+                    }
+                }
+            }
+            if (!ok) continue;
+            const u32x4 res = __builtin_bit_cast(u32x4, x);
+            if (r < a.Hq) {
+                reinterpret_cast<u32x4*>(static_cast<char*>(a.q_out) + ((int64_t)(t0 + tok) * a.Hq + r) * 256)[c] = res;
+            } else if (s_dst[tok] >= 0) {
+                const bool is_k = r < a.Hq + a.Hkv;
+                char* cache = static_cast<char*>(is_k ? a.k_cache : a.v_cache);
+                reinterpret_cast<u32x4*>(cache + s_dst[tok] + (r - a.Hq - (is_k ? 0 : a.Hkv)) * 256)[c] = res;
+            }
+        }
+    }
+}
+
+// ---- the accepted drafted tokens' rows ---------------------------------------------------------------
+//
+// A thread owns one 16-byte column of a sequence's token rows, in K or in V, and moves the list's rows in
+// order, kAcceptRows read before the first of them is written. The indices ascend, so index i of the list
+// is at least i: a row is written where rows of the list at or before it lay, never one still to be read.
+// So no thread waits for another, and the move is in place. Every wave checks the whole list first.
+constexpr int kAcceptThreads = 256;
+constexpr int kAcceptRows = 8;
+
+__global__ __launch_bounds__(kAcceptThreads) void accept_kv_kernel(AcceptArgs a) {
+    const int b = blockIdx.x, lane = threadIdx.x & 63;
+    const int row_pieces = a.Hkv * (kHeadDim / 8);
+    const int col = blockIdx.y * kAcceptThreads + threadIdx.x;
+    const int a0 = a.accepted_indptr[b], m = a.accepted_indptr[b + 1] - a0;
+    if (m <= 0) return;
+    const int pb = a.kv_indptr[b], np = a.kv_indptr[b + 1] - pb;
+    const int len = np > 0 ? (np - 1) * kPage + min(kPage, max(1, a.kv_last[b])) : 0;
+    const int n = a.q_indptr[b + 1] - a.q_indptr[b], ctx = len - n;
+    bool bad = n < 0 || ctx < 0;
+    for (int i = lane; i < m; i += 64) {
+        const int x = a.accepted[a0 + i];
+        bad |= x < 0 || x >= n || (i > 0 && a.accepted[a0 + i - 1] >= x);
+    }
+    if (__builtin_amdgcn_ballot_w64(bad)) {
+        if (col == 0 && a.n_invalid) atomicAdd(a.n_invalid, 1);
+        return;
+    }
+    if (col >= 2 * row_pieces) return;
+    u32x4* cache = reinterpret_cast<u32x4*>(col < row_pieces ? a.k_cache : a.v_cache);
+    const int piece = col < row_pieces ? col : col - row_pieces;
+    auto place = [&](int index) {
+        const int pos = ctx + index;
+        const size_t page = (size_t)(uint32_t)a.kv_indices[pb + pos / kPage];
+        return (page * kPage + pos % kPage) * row_pieces + piece;
+    };
+    for (int i0 = 0; i0 < m; i0 += kAcceptRows) {
+        u32x4 val[kAcceptRows];
+        int from[kAcceptRows];
+#pragma unroll
+        for (int u = 0; u < kAcceptRows; ++u) from[u] = a.accepted[a0 + min(i0 + u, m - 1)];
+#pragma unroll
+        for (int u = 0; u < kAcceptRows; ++u) val[u] = cache[place(from[u])];
+#pragma unroll
+        for (int u = 0; u < kAcceptRows; ++u)
+            if (i0 + u < m && from[u] != i0 + u) cache[place(i0 + u)] = val[u];
+    }
+}
+
 }  // namespace
+
+hipError_t launch_rope_append(const RopeArgs& args, int cus, hipStream_t s) {
+    RopeArgs a = args;
+    const int rows = a.Hq + 2 * a.Hkv;
+    if (a.n <= 0 || rows <= 0) return hipSuccess;
+    // one token per workgroup until every CU has some, then enough for kRopeRows rows per lane group
+    const int fill = kRopeRows * (kRopeThreads / 16) / rows;
+    a.tpb = std::max(1, std::min({kRopeMaxTokens, fill, a.n / std::max(1, 4 * cus)}));
+    a.rows_m = div_multiplier((uint32_t)rows);
+    rope_append_kernel<<<(a.n + a.tpb - 1) / a.tpb, kRopeThreads, 0, s>>>(a);
+    return hipGetLastError();
+}
+
+hipError_t launch_accept_kv(const AcceptArgs& a, hipStream_t s) {
+    if (a.B <= 0) return hipSuccess;
+    const int cols = 2 * a.Hkv * (kHeadDim / 8);
+    accept_kv_kernel<<<dim3(a.B, (cols + kAcceptThreads - 1) / kAcceptThreads), kAcceptThreads, 0, s>>>(a);
+    return hipGetLastError();
+}
 
 // Tokens per workgroup: enough workgroups for every CU first (a decode step's few tokens get one
 // each), then up to one full pass per thread (a prefill's many tokens).

@@ -478,3 +478,5 @@ int occupancy_cascade_prefix(int G) {
 }
 
 }  // namespace pdattn
+
+#include "tree_body.h"

@@ -158,6 +158,61 @@ struct AppendArgs {
     int tpb;                      // tokens per workgroup (set by launch_append_kv)
 };
 
+// Rotary positions and the paged append (pdattn_rope_append_kv).
+struct RopeArgs {
+    const void*    q;             // [n, Hq, 128] fp16, q_stride bytes from token to token; null with Hq = 0
+    const void*    k_new;         // [n, Hkv, 128], likewise
+    const void*    v_new;
+    void*          q_out;         // [n, Hq, 128]
+    void*          k_cache;       // [num_pages, 16, Hkv, 128]
+    void*          v_cache;
+    const int32_t* kv_indptr;
+    const int32_t* kv_indices;
+    const int32_t* batch_idx;
+    const int32_t* positions;
+    const int32_t* rope_positions;
+    const double*  freq;
+    int32_t*       n_invalid;
+    int64_t        q_stride, k_stride, v_stride;   // bytes
+    int            n, B, Hq, Hkv, rotary_dim, interleaved;
+    float          scale;
+    int            tpb;           // tokens per workgroup, and the multiplier of a token's rows (set by the launch)
+    uint32_t       rows_m;
+};
+
+// Accepted drafted tokens' rows to the front of their range (pdattn_accept_kv).
+struct AcceptArgs {
+    void*          k_cache;
+    void*          v_cache;
+    const int32_t* kv_indptr;
+    const int32_t* kv_indices;
+    const int32_t* kv_last;
+    const int32_t* q_indptr;
+    const int32_t* accepted_indptr;
+    const int32_t* accepted;
+    int32_t*       n_invalid;
+    int            B, Hkv;
+};
+
+// Attention of drafted tokens (pdattn_tree_attention).
+struct TreeArgs {
+    const _Float16* q;
+    const uint8_t*  k;
+    const uint8_t*  v;
+    const int32_t*  kv_indptr;
+    const int32_t*  kv_indices;
+    const int32_t*  kv_last;
+    const int32_t*  q_indptr;     // or null: one token per sequence
+    const uint32_t* mask;         // or null: chains
+    const int32_t*  depth;        // or null: the token's index
+    const float*    slopes;       // or null
+    _Float16*       out;
+    float*          lse;
+    int B, Hq, Hkv, G, n_tokens, mask_words, window, sink;
+    float scale_log2;             // sm_scale log2(e)
+    float cap_in, cap_out;        // sm_scale / cap and cap log2(e), or 0
+};
+
 // Arguments of the MFMA shared-prefix kernel.
 struct PrefixArgs {
     const _Float16* q;
@@ -202,6 +257,9 @@ hipError_t launch_fill_i32(int32_t* p, int32_t value, size_t n, hipStream_t s);
 hipError_t launch_cascade_prefix(const PrefixArgs& a, int G, hipStream_t s);
 hipError_t launch_cascade_step(const StepArgs& a, int G, int hp, hipStream_t s);
 hipError_t launch_append_kv(const AppendArgs& a, int cus, hipStream_t s);
+hipError_t launch_rope_append(const RopeArgs& a, int cus, hipStream_t s);
+hipError_t launch_accept_kv(const AcceptArgs& a, hipStream_t s);
+hipError_t launch_tree_attention(const TreeArgs& a, hipStream_t s);
 hipError_t launch_stream_read(const void* buf, size_t bytes, uint32_t* sink, int grid, hipStream_t s);
 hipError_t launch_flush(void* buf, size_t bytes, int grid, hipStream_t s);
 

@@ -49,6 +49,8 @@ EXPORTS = [
     "pdattn_cascade_decode", "pdattn_cascade_set_mode",
     "pdattn_cascade_plan_destroy",
     "pdattn_append_kv",
+    "pdattn_rope_frequencies", "pdattn_rope_append_kv",
+    "pdattn_tree_workspace_size", "pdattn_tree_attention", "pdattn_accept_kv",
     "pdattn_stream_read", "pdattn_flush_cache", "pdattn_get_device_info",
 ]
 
@@ -109,6 +111,45 @@ class CascadeInfo(ctypes.Structure):
 # pdattn_cascade_set_mode
 CASCADE_FUSED, CASCADE_SERIAL, CASCADE_TWO_STREAMS = 0, 1, 2
 RUN_DECODE, RUN_MERGE, RUN_ALL = 1, 2, 3   # pdattn_plan_run_part
+
+
+class RopeAppendParams(ctypes.Structure):
+    """pdattn_rope_append_params."""
+    _fields_ = [
+        ("q", ctypes.c_void_p), ("k_new", ctypes.c_void_p), ("v_new", ctypes.c_void_p),
+        ("q_out", ctypes.c_void_p), ("k_cache", ctypes.c_void_p), ("v_cache", ctypes.c_void_p),
+        ("kv_indptr", ctypes.c_void_p), ("kv_indices", ctypes.c_void_p),
+        ("batch_idx", ctypes.c_void_p), ("positions", ctypes.c_void_p),
+        ("rope_positions", ctypes.c_void_p), ("freq", ctypes.c_void_p),
+        ("n_invalid", ctypes.c_void_p),
+        ("q_stride", ctypes.c_int64), ("k_stride", ctypes.c_int64), ("v_stride", ctypes.c_int64),
+        ("n", ctypes.c_int32), ("B", ctypes.c_int32), ("Hq", ctypes.c_int32), ("Hkv", ctypes.c_int32),
+        ("rotary_dim", ctypes.c_int32), ("interleaved", ctypes.c_int32), ("scale", ctypes.c_float),
+    ]
+
+
+class ScoreParams(ctypes.Structure):
+    """pdattn_score_params."""
+    _fields_ = [("soft_cap", ctypes.c_float), ("slopes", ctypes.c_void_p),
+                ("window", ctypes.c_int32), ("sink", ctypes.c_int32)]
+
+
+class TreeParams(ctypes.Structure):
+    """pdattn_tree_params."""
+    _fields_ = [
+        ("q", ctypes.c_void_p), ("k_cache", ctypes.c_void_p), ("v_cache", ctypes.c_void_p),
+        ("kv_indptr", ctypes.c_void_p), ("kv_indices", ctypes.c_void_p),
+        ("kv_last_page_len", ctypes.c_void_p), ("q_indptr", ctypes.c_void_p),
+        ("mask", ctypes.c_void_p), ("depth", ctypes.c_void_p),
+        ("B", ctypes.c_int32), ("Hq", ctypes.c_int32), ("Hkv", ctypes.c_int32),
+        ("n_tokens", ctypes.c_int32), ("max_tokens", ctypes.c_int32), ("mask_words", ctypes.c_int32),
+        ("sm_scale", ctypes.c_float), ("score", ScoreParams),
+    ]
+
+
+# pdattn_rope_frequencies
+ROPE_PLAIN, ROPE_LINEAR, ROPE_BASE, ROPE_YARN, ROPE_WAVELENGTH = range(5)
+TREE_MAX_TOKENS = 512   # PDATTN_TREE_MAX_TOKENS
 
 
 class DeviceInfo(ctypes.Structure):
@@ -172,6 +213,11 @@ def lib():
         "pdattn_cascade_set_mode": ([P, I], I),
         "pdattn_cascade_plan_destroy": ([P], None),
         "pdattn_append_kv": ([P, P, P, P, P, P, P, P, I, I, I, P, P], I),
+        "pdattn_rope_frequencies": ([I] + [ctypes.c_double, I] + [ctypes.c_double] * 4 + [P, ctypes.POINTER(ctypes.c_float)], I),
+        "pdattn_rope_append_kv": ([ctypes.POINTER(RopeAppendParams), P], I),
+        "pdattn_tree_workspace_size": ([ctypes.POINTER(TreeParams)], S),
+        "pdattn_tree_attention": ([ctypes.POINTER(TreeParams), P, P, ctypes.POINTER(Workspace), P], I),
+        "pdattn_accept_kv": ([P, P, P, P, P, P, P, P, I, I, P, P], I),
         "pdattn_stream_read": ([P, S, P, P], I),
         "pdattn_flush_cache": ([P, S, P], I),
         "pdattn_get_device_info": ([ctypes.POINTER(DeviceInfo)], I),
@@ -413,6 +459,101 @@ def append_kv(k_new, v_new, k_cache, v_cache, kv_indptr, kv_indices, batch_idx, 
                                   ptr(kv_indices), ptr(batch_idx), ptr(positions), n, B, Hkv,
                                   ptr(n_invalid) if n_invalid is not None else None,
                                   stream_ptr(stream)), "pdattn_append_kv")
+
+
+# ---- rotary positions, drafted tokens, the accepted path -----------------------------------------
+
+def rope_frequencies(rotary_dim: int, base: float = 10000.0, scaling: int = ROPE_PLAIN, factor: float = 1.0,
+                     trained_len: float = 0.0, slow: float = 1.0, fast: float = 32.0):
+    """pdattn_rope_frequencies: (float64 array of rotary_dim / 2 frequencies, factor of cos and sin)."""
+    import numpy as np
+    f, sc = np.zeros(max(1, rotary_dim // 2)), ctypes.c_float()
+    _check(lib().pdattn_rope_frequencies(rotary_dim, base, scaling, factor, trained_len, slow, fast,
+                                         f.ctypes.data_as(ctypes.c_void_p), ctypes.byref(sc)),
+           "pdattn_rope_frequencies")
+    return f, sc.value
+
+
+def _rows(x, name):
+    """Heads and token stride (elements) of a [n, heads, 128] fp16 tensor with contiguous heads."""
+    if x.dim() != 3 or x.shape[2] != HEAD_DIM or x.element_size() != 2:
+        raise ValueError(f"{name} must be [n, heads, {HEAD_DIM}] fp16")
+    if x.shape[0] > 0 and (x.stride(2) != 1 or (x.shape[1] > 1 and x.stride(1) != HEAD_DIM)):
+        raise ValueError(f"the heads of a token of {name} must be contiguous")
+    return x.shape[1], x.stride(0)
+
+
+def make_rope_append_params(q, k_new, v_new, q_out, k_cache, v_cache, kv_indptr, kv_indices, batch_idx, positions,
+                            freq, B: int, rotary_dim: int = HEAD_DIM, interleaved: bool = False, scale: float = 1.0,
+                            rope_positions=None, n_invalid=None) -> RopeAppendParams:
+    """pdattn_rope_append_params from tensors: q (or None), k_new and v_new [n, heads, 128], possibly slices of
+    one tensor; freq float64 [rotary_dim / 2] on the device. The block holds addresses, and keeps the tensors alive."""
+    p = RopeAppendParams()
+    p.Hkv, p.k_stride = _rows(k_new, "k_new")
+    hv, p.v_stride = _rows(v_new, "v_new")
+    p.n = k_new.shape[0]
+    if q is not None:
+        p.Hq, p.q_stride = _rows(q, "q")
+        if q_out is None or tuple(q_out.shape) != tuple(q.shape) or not q_out.is_contiguous():
+            raise ValueError("q_out must be contiguous and shaped like q")
+    if hv != p.Hkv or v_new.shape[0] != p.n or (q is not None and q.shape[0] != p.n):
+        raise ValueError("q, k_new and v_new do not match")
+    if freq.element_size() != 8 or freq.numel() != rotary_dim // 2:
+        raise ValueError("freq must be float64 [rotary_dim / 2]")
+    for name, x in (("batch_idx", batch_idx), ("positions", positions), ("rope_positions", rope_positions)):
+        if x is not None and (x.numel() != p.n or x.element_size() != 4):
+            raise ValueError(f"{name} must be int32 [n]")
+    p.q, p.k_new, p.v_new, p.q_out = ptr(q), ptr(k_new), ptr(v_new), ptr(q_out) if q is not None else None
+    p.k_cache, p.v_cache = ptr(k_cache), ptr(v_cache)
+    p.kv_indptr, p.kv_indices = ptr(kv_indptr), ptr(kv_indices)
+    p.batch_idx, p.positions, p.rope_positions = ptr(batch_idx), ptr(positions), ptr(rope_positions)
+    p.freq, p.n_invalid = ptr(freq), ptr(n_invalid)
+    p.B, p.rotary_dim, p.interleaved, p.scale = B, rotary_dim, int(bool(interleaved)), scale
+    p.keep = (q, k_new, v_new, q_out, k_cache, v_cache, kv_indptr, kv_indices, batch_idx, positions, freq, rope_positions,
+              n_invalid)
+    return p
+
+
+def rope_append_kv(p: RopeAppendParams, stream=None):
+    """pdattn_rope_append_kv: rotate q into q_out and k, and append k and v to the paged cache."""
+    _check(lib().pdattn_rope_append_kv(ctypes.byref(p), stream_ptr(stream)), "pdattn_rope_append_kv")
+
+
+def make_tree_params(q, k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len, B: int, Hq: int, Hkv: int,
+                     q_indptr=None, max_tokens: int = 1, mask=None, depth=None, sm_scale=None, soft_cap: float = 0.0,
+                     slopes=None, window: int = 0, sink: int = 0, n_tokens=None, mask_words=None) -> TreeParams:
+    """pdattn_tree_params. n_tokens and mask_words come from the shapes of q [n_tokens, Hq, 128] and mask
+    [n_tokens, words] (int32 bits) unless they are given. The block holds addresses, and keeps the tensors alive."""
+    p = TreeParams()
+    p.q, p.k_cache, p.v_cache = ptr(q), ptr(k_cache), ptr(v_cache)
+    p.kv_indptr, p.kv_indices, p.kv_last_page_len = ptr(kv_indptr), ptr(kv_indices), ptr(kv_last_page_len)
+    p.q_indptr, p.mask, p.depth = ptr(q_indptr), ptr(mask), ptr(depth)
+    p.B, p.Hq, p.Hkv = B, Hq, Hkv
+    p.n_tokens = q.shape[0] if n_tokens is None else n_tokens
+    p.max_tokens = max_tokens
+    p.mask_words = (0 if mask is None else mask.shape[1]) if mask_words is None else mask_words
+    p.sm_scale = _SCALE if sm_scale is None else sm_scale
+    p.score = ScoreParams(soft_cap, ptr(slopes), window, sink)
+    p.keep = (q, k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len, q_indptr, mask, depth, slopes)
+    return p
+
+
+def tree_workspace_size(p: TreeParams) -> int:
+    return int(lib().pdattn_tree_workspace_size(ctypes.byref(p)))
+
+
+def tree_attention(p: TreeParams, out, lse, ws: Workspace, stream=None):
+    """pdattn_tree_attention: attention of drafted tokens (or of one token per sequence with changed scores)."""
+    _check(lib().pdattn_tree_attention(ctypes.byref(p), ptr(out), ptr(lse), ctypes.byref(ws), stream_ptr(stream)),
+           "pdattn_tree_attention")
+
+
+def accept_kv(k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len, q_indptr, accepted_indptr, accepted,
+              B: int, Hkv: int, n_invalid=None, stream=None):
+    """pdattn_accept_kv: the accepted drafted tokens' rows to the front of each sequence's drafted range."""
+    _check(lib().pdattn_accept_kv(ptr(k_cache), ptr(v_cache), ptr(kv_indptr), ptr(kv_indices),
+                                  ptr(kv_last_page_len), ptr(q_indptr), ptr(accepted_indptr), ptr(accepted), B, Hkv,
+                                  ptr(n_invalid), stream_ptr(stream)), "pdattn_accept_kv")
 
 
 # ---- cascade ---------------------------------------------------------------------------------

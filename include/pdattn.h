@@ -360,6 +360,125 @@ int pdattn_append_kv(const void* k_new, const void* v_new, void* k_cache, void* 
                      const int32_t* positions, int n, int B, int Hkv, int32_t* n_invalid,
                      void* stream);
 
+/* ---- rotary positions and the paged append ------------------------------------------------- */
+
+/* How the rotary frequencies are scaled for contexts longer than the trained one (`factor` times). */
+enum {
+    PDATTN_ROPE_PLAIN = 0,      /* f_i = base^(-2 i / rotary_dim)                                     */
+    PDATTN_ROPE_LINEAR = 1,     /* f_i / factor (positions divided)                                   */
+    PDATTN_ROPE_BASE = 2,       /* the plain f_i of base * factor^(rotary_dim / (rotary_dim - 2))     */
+    PDATTN_ROPE_YARN = 3,       /* YaRN: f_i / factor for pairs that turn fewer than `slow` times in
+                                   `trained_len` positions, f_i for more than `fast`, a linear ramp
+                                   over the pair index between; cos and sin times 0.1 ln(factor) + 1 */
+    PDATTN_ROPE_WAVELENGTH = 4  /* the same with a ramp linear in the number of turns, between `slow`
+                                   and `fast` turns; cos and sin unscaled                             */
+};
+
+/* Host helper: the rotary_dim / 2 frequencies (radians per position) in 64 bits into h_freq, and the
+ * factor of cos and sin into *attn_scale. rotary_dim even in [2, 128], base > 1, factor >= 1; trained_len,
+ * slow and fast are used by YARN and WAVELENGTH only (0 < slow < fast; YaRN's own are 1 and 32).
+ * BASE with rotary_dim = 2 has one pair, of frequency 1 whatever the base. */
+int pdattn_rope_frequencies(int rotary_dim, double base, int scaling, double factor, double trained_len,
+                            double slow, double fast, double* h_freq, float* attn_scale);
+
+/* One launch for the step before the attention: rotate the new tokens' q and k, and append k and v to
+ * the paged cache (pdattn_append_kv's rules: the page table already covers the tokens; a token whose
+ * sequence or position is out of range is not written and counted in *n_invalid, which the caller
+ * zeroes). Pair i of a head's first rotary_dim dims, (u, w) = dims (i, i + rotary_dim / 2), or (2 i,
+ * 2 i + 1) if interleaved, becomes scale * (u cos a - w sin a, w cos a + u sin a), a = p * freq[i],
+ * p = rope_positions[t], or positions[t] where that is NULL. The angle is formed and reduced in 64
+ * bits, so far positions lose nothing; the results are rounded to fp16 once. The other dims are
+ * copied. q_out is written for every token, one that is not appended included.
+ * q, k_new and v_new are [n, heads, 128] fp16 with *_stride elements from token to token (the heads of
+ * a token contiguous), so the three may be slices of one projection's output. q_out [n, Hq, 128] is
+ * contiguous and may be q itself (then q_stride = Hq * 128); it may not overlap q otherwise. q = NULL
+ * (with Hq = 0): only k and v. Pointers and strides are multiples of 16 bytes. */
+typedef struct pdattn_rope_append_params {
+    const void*    q;
+    const void*    k_new;
+    const void*    v_new;
+    void*          q_out;
+    void*          k_cache;
+    void*          v_cache;
+    const int32_t* kv_indptr;
+    const int32_t* kv_indices;
+    const int32_t* batch_idx;       /* [n] sequence of each token                        */
+    const int32_t* positions;       /* [n] its position in the cache                     */
+    const int32_t* rope_positions;  /* [n] its rotary position, or NULL: positions       */
+    const double*  freq;            /* device [rotary_dim / 2]                           */
+    int32_t*       n_invalid;       /* device, optional                                  */
+    int64_t        q_stride, k_stride, v_stride;
+    int32_t        n, B, Hq, Hkv;
+    int32_t        rotary_dim;      /* even, 2 .. 128                                    */
+    int32_t        interleaved;
+    float          scale;           /* factor of cos and sin (1: none)                   */
+} pdattn_rope_append_params;
+int pdattn_rope_append_kv(const pdattn_rope_append_params* p, void* stream);
+
+/* ---- attention of drafted tokens over the cache -------------------------------------------- */
+
+/* What changes a score x = sm_scale * q.k before the softmax, in this order. All zero: nothing. */
+typedef struct pdattn_score_params {
+    float        soft_cap;   /* > 0: x becomes soft_cap * tanh(x / soft_cap)                         */
+    const float* slopes;     /* device [Hq] or NULL: slope[h] * (key's position - query's) is added  */
+    int32_t      window;     /* > 0: a key `window` or more positions before the query is not seen   */
+    int32_t      sink;       /* with a window: the first `sink` keys of the sequence are seen anyway */
+} pdattn_score_params;
+
+#define PDATTN_TREE_MAX_TOKENS 512   /* tokens of a sequence where mask or depth is given */
+
+/* Attention of several query tokens per sequence over the paged cache: the verification of drafted
+ * tokens (speculative decoding), a chunk of a prefill over a cached context, or, with q_indptr = NULL,
+ * the decode of one token per sequence with changed scores.
+ * The tokens q_indptr[b] .. q_indptr[b + 1] of q are the last n_b of the len_b cached tokens of
+ * sequence b, in order (append them first): token i of them is cached at ctx_b + i, ctx_b = len_b - n_b.
+ * It sees the keys below ctx_b, and of the others key ctx_b + j
+ *   - if bit j of its mask row is set (word j / 32, bit j % 32; bits past mask_words * 32 count as 0):
+ *     for a tree, its ancestors and itself;
+ *   - without a mask, if j <= i (a chain).
+ * Positions, for slopes and window: key t < ctx_b is at t, token i (as a query and as a key) at
+ * ctx_b + depth[i], or ctx_b + i without depth; a depth below 0 counts as 0.
+ * A token that sees no key gets out = 0, lse = -inf. Keys that a token does not see have no influence
+ * on it, whatever bits they hold. Rows of q, out and lse from q_indptr[B] on are neither read nor written.
+ * Nothing on the host depends on the lengths, the trees or q_indptr, so a captured call can be replayed
+ * with others; max_tokens, the most tokens of any sequence, only chooses the kernel: results do not
+ * depend on it beyond the order of sums. Where mask or depth is given it may not pass
+ * PDATTN_TREE_MAX_TOKENS: drafted keys of a sequence past that many are then not seen. */
+typedef struct pdattn_tree_params {
+    const void*     q;                  /* [n_tokens, Hq, 128] fp16                            */
+    const void*     k_cache;
+    const void*     v_cache;
+    const int32_t*  kv_indptr;
+    const int32_t*  kv_indices;
+    const int32_t*  kv_last_page_len;
+    const int32_t*  q_indptr;           /* device [B + 1], or NULL: one token per sequence     */
+    const uint32_t* mask;               /* device [n_tokens, mask_words], or NULL: chains      */
+    const int32_t*  depth;              /* device [n_tokens], or NULL: the token's index       */
+    int32_t         B, Hq, Hkv, n_tokens, max_tokens, mask_words;
+    float           sm_scale;
+    pdattn_score_params score;
+} pdattn_tree_params;
+
+/* Workspace bytes pdattn_tree_attention needs for `p` (0 on an invalid `p`). They depend on the device
+ * and on B, Hq, Hkv, n_tokens and max_tokens alone. */
+size_t pdattn_tree_workspace_size(const pdattn_tree_params* p);
+/* out [n_tokens, Hq, 128] fp16 and lse [n_tokens, Hq] fp32; the workspace as in
+ * pdattn_decode_attention. */
+int pdattn_tree_attention(const pdattn_tree_params* p, void* out, float* lse, pdattn_workspace* ws,
+                          void* stream);
+
+/* Keep the accepted drafted tokens of every sequence: their rows move to the front of the drafted
+ * range, K and V, all kv heads, in place. accepted[accepted_indptr[b] + i] is the index (0 .. n_b - 1, as
+ * in pdattn_tree_attention) of the i-th token accepted, strictly ascending in i, as the nodes of a path
+ * are; its row goes from position ctx_b + that index to ctx_b + i. The page table and q_indptr are
+ * those of the attention, and the caller shortens the sequence to ctx_b + accepted afterwards. A sequence
+ * whose list does not ascend or leaves its tokens is left as it was and counted in *n_invalid (device,
+ * optional, zeroed by the caller). Sequences may not share the pages that hold drafted tokens. */
+int pdattn_accept_kv(void* k_cache, void* v_cache, const int32_t* kv_indptr, const int32_t* kv_indices,
+                     const int32_t* kv_last_page_len, const int32_t* q_indptr,
+                     const int32_t* accepted_indptr, const int32_t* accepted, int B, int Hkv,
+                     int32_t* n_invalid, void* stream);
+
 /* ---- measurement helpers ------------------------------------------------------------------ */
 
 /* Streams `bytes` (a multiple of 16) with 16-byte loads and folds them into one word, written

@@ -216,3 +216,153 @@ def append_kv(k_cache, v_cache, k_new, v_new, batch_idx, positions, indptr, indi
         vc[page, slot] = v_new[t]
     return kc, vc, bad
 
+
+
+# ---- drafted tokens -----------------------------------------------------------------------------
+
+TREE_FAULTS = ("none", "mask_transposed", "chain_excludes_self", "context_shifted", "bias_before_cap", "bias_sign",
+               "window_inclusive", "sink_in_window_only", "slot_positions", "group_modulo")
+
+
+def _sequence(indptr, indices, last, b):
+    """Page ids and length of sequence b (a last-page length outside [1, 16] is clamped)."""
+    pages = np.asarray(indices)[int(indptr[b]):int(indptr[b + 1])]
+    return pages, (len(pages) - 1) * PAGE + min(PAGE, max(1, int(last[b]))) if len(pages) else 0
+
+
+def tree_attention(q, k, v, indptr, indices, last, Hq: int, Hkv: int, q_indptr=None, mask=None, depth=None,
+                   sm_scale=None, soft_cap: float = 0.0, slopes=None, window: int = 0, sink: int = 0,
+                   max_tokens: int = 512, fault: str = "none"):
+    """Attention of drafted tokens in 64 bits, from the definition: token i of sequence b, cached at ctx + i
+    (ctx = length - tokens), sees every key below ctx and key ctx + j if bit j of its mask row is set (j <= i
+    without a mask); scores sm_scale q.k, capped by cap tanh(x / cap), plus slope (key position - query
+    position), positions being ctx + depth (the index without depths, a negative one 0); with a window only keys
+    less than it before the query, or below `sink`. Keys not seen are not read.
+
+    Returns (out [n, Hq, 128], lse [n, Hq], slack) where slack holds what a 32-bit evaluation's error is
+    proportional to: "weight" [n, Hq, 128] = sum p |v|; "score" [n, Hq] = sum p e and "score_v" [n, Hq, 128] =
+    sum p e |v|, e being a score's error bound in units of 2^-24: 136 sum_d |q_d k_d| sm_scale (the products'
+    sum) + 16 (|x| + |bias|) (what follows it); "keys" [n, Hq] the keys seen. Tokens of no sequence: NaN.
+    `fault` plants a mistake for the tests that pin this function."""
+    q = np.asarray(q).astype(np.float64)
+    n_tokens = q.shape[0]
+    B, G = len(indptr) - 1, Hq // Hkv
+    q_indptr = np.arange(B + 1) if q_indptr is None else np.asarray(q_indptr)
+    sm = 1.0 / np.sqrt(HEAD_DIM) if sm_scale is None else sm_scale
+    out, lse = np.full((n_tokens, Hq, HEAD_DIM), np.nan), np.full((n_tokens, Hq), np.nan)
+    slack = {"weight": np.zeros_like(out), "score": np.zeros_like(lse), "score_v": np.zeros_like(out),
+             "keys": np.zeros_like(lse)}
+    for b in range(B):
+        pages, length = _sequence(indptr, indices, last, b)
+        q0, n = int(q_indptr[b]), int(q_indptr[b + 1]) - int(q_indptr[b])
+        ctx = length - n + (1 if fault == "context_shifted" else 0)
+        flat = np.repeat(np.asarray(pages, np.int64) * PAGE, PAGE) + np.tile(np.arange(PAGE), len(pages))
+        flat = flat[:length]
+        dep = np.arange(n) if depth is None or fault == "slot_positions" else np.maximum(0, np.asarray(depth)[q0:q0 + n])
+        j = np.arange(length) - ctx
+        drafted = j >= 0
+        # position of every key relative to ctx
+        pos_k = np.where(drafted, dep[np.clip(j, 0, max(n - 1, 0))] if n else 0, j)
+        look = []   # per token: which keys it sees, and how far before it they are
+        for i in range(n):
+            if mask is None:
+                seen = ~drafted | (j <= i - (1 if fault == "chain_excludes_self" else 0))
+            else:
+                m = np.asarray(mask).view(np.uint32)
+                jj = np.clip(j, 0, 32 * m.shape[1] - 1)
+                bits = m[q0 + i, jj // 32] >> (jj % 32) & 1
+                if fault == "mask_transposed":
+                    jj = np.clip(jj, 0, n - 1)
+                    bits = m[q0 + jj, i // 32] >> np.uint32(i % 32) & 1
+                seen = ~drafted | ((bits != 0) & (j < 32 * m.shape[1]))
+            if mask is not None or depth is not None:
+                seen &= j < max_tokens
+            apart = dep[i] - pos_k
+            if window > 0:
+                near = apart < window + (1 if fault == "window_inclusive" else 0)
+                seen &= near if fault == "sink_in_window_only" else near | (np.arange(length) < sink)
+            look.append((i, apart, np.flatnonzero(seen)))
+        for kvh in range(Hkv):
+            heads = [h for h in range(Hq) if (h % Hkv if fault == "group_modulo" else h // G) == kvh]
+            kb = np.asarray(k).reshape(-1, Hkv, HEAD_DIM)[flat, kvh].astype(np.float64)
+            vb = np.asarray(v).reshape(-1, Hkv, HEAD_DIM)[flat, kvh].astype(np.float64)
+            for i, apart, at in look:
+                t = q0 + i
+                if len(at) == 0:
+                    out[t, heads], lse[t, heads] = 0.0, -np.inf
+                    continue
+                kk, vv = (kb, vb) if len(at) == length else (kb[at], vb[at])
+                for h in heads:
+                    x = kk @ q[t, h] * sm
+                    e = 136 * (np.abs(kk) @ np.abs(q[t, h])) * abs(sm)
+                    bias = np.zeros(len(at)) if slopes is None else float(slopes[h]) * -apart[at]
+                    if fault == "bias_sign":
+                        bias = -bias
+                    if fault == "bias_before_cap":
+                        x = x + bias
+                    if soft_cap > 0:
+                        x = soft_cap * np.tanh(x / soft_cap)
+                    if fault != "bias_before_cap":
+                        x = x + bias
+                    e = e + 16 * (np.abs(x) + np.abs(bias))
+                    top = x.max()
+                    w = np.exp(x - top)
+                    p = w / w.sum()
+                    out[t, h], lse[t, h] = p @ vv, top + np.log(w.sum())
+                    slack["weight"][t, h] = p @ np.abs(vv)
+                    slack["score"][t, h], slack["score_v"][t, h] = p @ e, (p * e) @ np.abs(vv)
+                    slack["keys"][t, h] = len(at)
+    return out, lse, slack
+
+
+ROPE_FAULTS = ("none", "other_pairing", "sign", "half_of_head", "scale_twice")
+
+
+def rope(x, positions, freq, rotary_dim: int, interleaved: bool = False, scale: float = 1.0, fault: str = "none"):
+    """Rotary positions in 64 bits: pair (u, w) of the first rotary_dim dims of x [n, heads, 128], at angle
+    a = position * freq, becomes scale (u cos a - w sin a, w cos a + u sin a)."""
+    x = np.asarray(x).astype(np.float64)
+    y = x.copy()
+    if fault == "other_pairing":
+        interleaved = not interleaved
+    if fault == "half_of_head":
+        rotary_dim = min(HEAD_DIM, 2 * rotary_dim)
+        freq = np.resize(freq, rotary_dim // 2)
+    for t, p in enumerate(np.asarray(positions)):
+        for i in range(rotary_dim // 2):
+            u, w = (2 * i, 2 * i + 1) if interleaved else (i, i + rotary_dim // 2)
+            a = float(p) * float(freq[i]) * (-1 if fault == "sign" else 1)
+            s = scale * scale if fault == "scale_twice" else scale
+            y[t, :, u] = s * (x[t, :, u] * np.cos(a) - x[t, :, w] * np.sin(a))
+            y[t, :, w] = s * (x[t, :, w] * np.cos(a) + x[t, :, u] * np.sin(a))
+    return y
+
+
+ACCEPT_FAULTS = ("none", "from_the_front", "keys_only", "descending")
+
+
+def accept_kv(k_cache, v_cache, indptr, indices, last, q_indptr, accepted_indptr, accepted, fault: str = "none"):
+    """The rows of the accepted drafted tokens to the front of each sequence's drafted range: list entry i of
+    sequence b moves position ctx + accepted[i] to ctx + i. A list that does not ascend within the sequence's
+    tokens is counted and its sequence left alone. Returns (k_cache', v_cache', n_invalid)."""
+    kc, vc = np.array(k_cache, copy=True), np.array(v_cache, copy=True)
+    bad = 0
+    for b in range(len(indptr) - 1):
+        lst = np.asarray(accepted)[int(accepted_indptr[b]):int(accepted_indptr[b + 1])].astype(np.int64)
+        if len(lst) == 0:
+            continue
+        pages, length = _sequence(indptr, indices, last, b)
+        n = int(q_indptr[b + 1]) - int(q_indptr[b])
+        ctx = length - n
+        if n < 0 or ctx < 0 or lst.min() < 0 or lst.max() >= n or np.any(np.diff(lst) <= 0):
+            bad += 1
+            continue
+        base = 0 if fault == "from_the_front" else ctx
+        order = range(len(lst) - 1, -1, -1) if fault == "descending" else range(len(lst))
+        for i in order:
+            src, dst = ctx + lst[i], base + i
+            s, d = (pages[src // PAGE], src % PAGE), (pages[dst // PAGE], dst % PAGE)
+            kc[d] = kc[s]
+            if fault != "keys_only":
+                vc[d] = vc[s]
+    return kc, vc, bad
