@@ -1638,6 +1638,26 @@ int check_tree_params(const pdattn_tree_params* p, int* G) {
     return PDATTN_OK;
 }
 
+// The launch of pdattn_tree_attention: rows per workgroup, ranges, and the workspace.
+struct TreeLayout {
+    int rows = 16, ranges = 1;
+    size_t off_plse = 0, off_po = 0, bytes = 0;
+};
+
+int tree_layout(const pdattn_tree_params* p, int G, TreeLayout* L) {
+    DeviceFacts f;
+    if (int st = device_facts(&f)) return st;
+    const int64_t rows = (int64_t)(p->q_indptr ? p->max_tokens : 1) * G;
+    L->rows = rows <= 16 ? 16 : 32;
+    L->ranges = std::max(1, 2 * f.cus / p->Hkv);
+    const size_t slots = (size_t)2 * L->ranges * p->Hkv * L->rows;
+    size_t off = align_up(sizeof(int4) * L->ranges);
+    L->off_plse = off; off += align_up(sizeof(float) * slots);
+    L->off_po = off;   off += align_up(sizeof(float) * slots * kHeadDim);
+    L->bytes = off;
+    return PDATTN_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -1645,7 +1665,8 @@ extern "C" {
 size_t pdattn_tree_workspace_size(const pdattn_tree_params* p) {
     int G = 0;
     if (check_tree_params(p, &G) != PDATTN_OK || p->B == 0 || p->n_tokens == 0) return 0;
-    return kAlign;
+    TreeLayout L;
+    return tree_layout(p, G, &L) == PDATTN_OK ? L.bytes : 0;
 }
 
 int pdattn_tree_attention(const pdattn_tree_params* p, void* out, float* lse, pdattn_workspace* ws,
@@ -1655,9 +1676,11 @@ int pdattn_tree_attention(const pdattn_tree_params* p, void* out, float* lse, pd
     if (p->B == 0 || p->n_tokens == 0) return PDATTN_OK;
     if (!out || !lse) return fail(PDATTN_ERR_INVALID_ARGUMENT, "null out / lse");
     if (!aligned16(out)) return fail(PDATTN_ERR_INVALID_ARGUMENT, "out must be 16-byte aligned");
-    const size_t need = pdattn_tree_workspace_size(p);
-    if (int st = ensure_ws(ws, need)) return st;
-    res_written(ws->base, need);
+    TreeLayout L;
+    if (int st = tree_layout(p, G, &L)) return st;
+    if (int st = ensure_ws(ws, L.bytes)) return st;
+    char* base = static_cast<char*>(ws->base);
+    res_written(base, L.bytes);
     res_written_outputs(out, lse, (size_t)p->n_tokens * p->Hq);
     TreeArgs a;
     a.q = static_cast<const _Float16*>(p->q);
@@ -1676,10 +1699,18 @@ int pdattn_tree_attention(const pdattn_tree_params* p, void* out, float* lse, pd
     a.Hq = p->Hq;
     a.Hkv = p->Hkv;
     a.G = G;
+    a.cuts = reinterpret_cast<int4*>(base);
+    a.part_lse = reinterpret_cast<float*>(base + L.off_plse);
+    a.part_o = reinterpret_cast<float*>(base + L.off_po);
     a.n_tokens = p->n_tokens;
+    a.max_tokens = p->q_indptr ? p->max_tokens : 1;
     a.mask_words = p->mask_words;
-    a.window = p->score.window;
-    a.sink = p->score.sink;
+    a.rows = L.rows;
+    a.tpg = L.rows / G;
+    a.ranges = L.ranges;
+    a.least_units = 8;
+    a.window = std::min(p->score.window, 1 << 30);   // (past any position: sums of positions fit an int)
+    a.sink = std::min(p->score.sink, 1 << 30);
     a.scale_log2 = p->sm_scale * 1.4426950408889634f;
     a.cap_in = p->score.soft_cap > 0.f ? p->sm_scale / p->score.soft_cap : 0.f;
     a.cap_out = p->score.soft_cap * 1.4426950408889634f;

@@ -2,6 +2,8 @@
 // (prefix chunk or tree item, query group, kv head). The 4-wave body (prefix_body.h) serves tree
 // items and prefixes with up to 128 rows per kv head; a single prefix with more rows runs on the
 // 8-wave key-split body below.
+#include <algorithm>
+
 #include "timeline.h"
 
 PD_TIMELINE_TABLE(prefix)

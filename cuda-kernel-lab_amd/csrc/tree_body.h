@@ -5,129 +5,774 @@
 //   x = sm_scale q.k;  x = cap tanh(x / cap);  x += slope_h (pos_k - pos_q);  unseen: -inf
 //   out = sum_k softmax(x)_k v_k,  lse = ln sum_k exp(x_k)
 //
-// One wave per (token, query head): 64 keys at a time, a key per lane for the scores, two dims per lane
-// for the output.
+// The rows of a sequence for one kv head (its tokens times the head's G query heads) are the columns of fp16 MFMAs, as
+// in decode_body.h: S^T = K Q^T, O^T += V^T P^T, 16 rows a tile. A workgroup takes up to 16 NT rows; its four waves
+// split the keys, each streaming its own 32-key blocks through its own LDS slot by direct loads, with no barrier in
+// the loop; at the end of a piece the four states are joined through LDS. Which workgroup does what: tree_arith.h; the
+// device finds it from the page table and q_indptr, so that a captured launch serves any lengths.
 #pragma once
 
 #include <math.h>
 
-#include "pdattn_internal.h"
+#include "decode_body.h"
+#include "tree_arith.h"
 
 namespace pdattn {
 namespace {
 
 constexpr float kTreeLn2 = 0.69314718055994531f;
+constexpr float kTreeLog2e = 1.4426950408889634f;
 constexpr int kTreeMaxTokens = PDATTN_TREE_MAX_TOKENS;
+constexpr int kTreeMaskWords = kTreeMaxTokens / 32;
+constexpr int kTreeWaves = 4;
+constexpr int kTreeThreads = kTreeWaves * 64;
+constexpr int kTreeScan = 4;   // sequences per thread of a pass of the scan
 
-// tanh(x) in 32 bits. |x| <= 1: the fifth convergent of x / (1 + x^2 / (3 + x^2 / (5 + ...))) (Lambert), of
-// which 32 bits show no error; else 1 - 2 / (e^(2 |x|) + 1), whose 1 no longer cancels.
-__device__ __forceinline__ float tree_tanh(float x) {
-    const float z = x * x, t = fabsf(x);
-    const float small = x * fmaf(z, fmaf(z, 21.f, 1260.f), 10395.f) /
-                        fmaf(z, fmaf(z, z + 210.f, 4725.f), 10395.f);
-    const float e = __builtin_amdgcn_exp2f(2.8853900817779268f * t);
-    const float big = copysignf(1.f - 2.f / (e + 1.f), x);
-    return t <= 1.f ? small : big;
+// tanh(x) in 32 bits. |x| <= 1: the convergent x (10395 + 1260 z + 21 z^2) / (10395 + 4725 z + 210 z^2 + z^3), z = x^2, of
+// x / (1 + x^2 / (3 + x^2 / (5 + ...))) (Lambert), within 5e-10 of it; else 1 - 2 / (e^(2 |x|) + 1), whose 1 no
+// longer cancels.
+__device__ __forceinline__ float tree_tanh_small(float x) {
+    const float z = x * x;
+    return x * fmaf(z, fmaf(z, 21.f, 1260.f), 10395.f) *
+           __builtin_amdgcn_rcpf(fmaf(z, fmaf(z, z + 210.f, 4725.f), 10395.f));
+}
+__device__ __forceinline__ float tree_tanh_large(float x) {
+    const float e = __builtin_amdgcn_exp2f(2.8853900817779268f * fabsf(x));
+    return copysignf(fmaf(-2.f, __builtin_amdgcn_rcpf(e + 1.f), 1.f), x);
 }
 
-// Reductions over a wave, left in every lane.
-template <bool MAX>
-__device__ __forceinline__ float tree_wave_reduce(float v) {
+// The kernel's arguments, read again from the kernarg segment where they are used: held in scalar registers
+// across a piece they would spill. (Only valid in a kernel's own body, so in force-inlined functions alone.)
+typedef const __attribute__((address_space(4))) TreeArgs* TreeArgPtr;
+__device__ __forceinline__ TreeArgPtr tree_args() {
+    TreeArgPtr p = (TreeArgPtr)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return p;
+}
+
+// ---- the range of a workgroup ---------------------------------------------------------------------
+
+struct TreeScan {
+    int64_t wave[kTreeWaves];
+    int64_t prefix;   // units before the range's first sequence
+    int first;        // that sequence
+};
+
+template <class A>
+__device__ __forceinline__ TreeSeq tree_load_seq(const A& a, int b, int* q0, int* pb) {
+    const int ip0 = a.kv_indptr[b], ip1 = a.kv_indptr[b + 1], last = a.kv_last[b];
+    const int s0 = a.q_indptr ? a.q_indptr[b] : b, s1 = a.q_indptr ? a.q_indptr[b + 1] : b + 1;
+    *q0 = max(s0, 0);
+    *pb = ip0;
+    return tree_seq(ip0, ip1, last, s0, s1, a.n_tokens, a.tpg, a.window, a.sink);
+}
+
+__device__ __forceinline__ int64_t tree_shfl_up(int64_t v, int d) {
+    const int lo = __shfl_up((int)v, d, 64), hi = __shfl_up((int)(v >> 32), d, 64);
+    return (int64_t)(((uint64_t)(uint32_t)hi << 32) | (uint32_t)lo);
+}
+
+// Units of sequences 4 t .. 4 t + 3 of a pass (t = thread), the units before them in the pass, and the pass's sum.
+__device__ __forceinline__ int64_t tree_scan_pass(const TreeArgs& a, TreeScan& S, int b0, int64_t (&u)[kTreeScan], int64_t& sum) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    int64_t mine = 0;
+#pragma unroll
+    for (int k = 0; k < kTreeScan; ++k) {
+        const int b = b0 + kTreeScan * tid + k;
+        int q0, pb;
+        const TreeSeq t = tree_load_seq(a, min(b, a.B - 1), &q0, &pb);
+        u[k] = b < a.B ? t.total() : 0;
+        mine += u[k];
+    }
+    int64_t x = mine;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
-        const float o = __shfl_xor(v, d, 64);
-        v = MAX ? fmaxf(v, o) : v + o;
+        const int64_t y = tree_shfl_up(x, d);
+        if (lane >= d) x += y;
     }
+    if (lane == 63) S.wave[wave] = x;
+    __syncthreads();
+    int64_t before = 0;
+    sum = 0;
+#pragma unroll
+    for (int w = 0; w < kTreeWaves; ++w) {
+        before += w < wave ? S.wave[w] : 0;
+        sum += S.wave[w];
+    }
+    __syncthreads();
+    return before + x - mine;
+}
+
+// The units [lo, hi) of range g, and where they start (in S). False: there is no such range.
+__device__ __forceinline__ bool tree_find_range(const TreeArgs& a, TreeScan& S, int g, int64_t& lo, int64_t& hi, int64_t& units, int& ranges) {
+    constexpr int kPass = kTreeScan * kTreeThreads;
+    int64_t u[kTreeScan], sum, at = tree_scan_pass(a, S, 0, u, sum);
+    units = sum;
+    for (int b0 = kPass; b0 < a.B; b0 += kPass) {
+        (void)tree_scan_pass(a, S, b0, u, sum);
+        units += sum;
+    }
+    ranges = units > 0 ? tree_ranges(units, a.ranges, a.least_units) : 0;
+    if (g >= ranges) return false;
+    lo = tree_range_start(units, ranges, g);
+    hi = tree_range_start(units, ranges, g + 1);
+    int64_t before = 0;
+    for (int b0 = 0; b0 < a.B; b0 += kPass) {
+        if (a.B > kPass) at = tree_scan_pass(a, S, b0, u, sum);
+        int64_t p = before + at;
+#pragma unroll
+        for (int k = 0; k < kTreeScan; ++k) {
+            if (p <= lo && lo < p + u[k]) {
+                S.prefix = p;
+                S.first = b0 + kTreeScan * (int)threadIdx.x + k;
+            }
+            p += u[k];
+        }
+        before += sum;
+    }
+    __syncthreads();
+    return true;
+}
+
+// ---- one piece ------------------------------------------------------------------------------------
+
+template <int NT>
+struct TreeShared {
+    static constexpr int ROWS = 16 * NT;
+    alignas(256) uint8_t slot[kTreeWaves][kDecSlotBytes];   // a block of the wave's; at the end its output
+    float m[kTreeWaves][ROWS];
+    float l[kTreeWaves][ROWS];
+    uint32_t mask[ROWS][kTreeMaskWords];                    // the group's mask rows
+    int depth[kTreeMaxTokens];                              // the sequence's drafted tokens' depths
+    TreeScan scan;
+    int wild;                                               // the piece goes row by row (tree_piece_rows)
+};
+static_assert(TreeShared<2>::ROWS * kHeadDim * 4 <= kDecSlotBytes, "a wave's output fits its slot");
+
+// The value itself, as a new value in every call: what is formed from it is not kept across the loop.
+__device__ __forceinline__ uint32_t tree_fresh(uint32_t v) {
+    asm volatile("" : "+v"(v));
     return v;
 }
 
-constexpr int kTreeWaves = 4;
+__device__ __forceinline__ uint32_t tree_fresh_s(uint32_t v) {
+    asm volatile("" : "+s"(v));
+    return v;
+}
 
-__global__ __launch_bounds__(kTreeWaves * 64) void tree_rows_kernel(TreeArgs a) {
-    __shared__ float s_q[kTreeWaves][kHeadDim];
-    __shared__ float s_p[kTreeWaves][64];
-    __shared__ int s_off[kTreeWaves][64];
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int row = blockIdx.x * kTreeWaves + wave;
-    const bool live = row < a.n_tokens * a.Hq;
-    const int t = live ? row / a.Hq : 0, h = live ? row - t * a.Hq : 0, kvh = h / a.G;
-    // the token's sequence: the first b with q_indptr[b + 1] > t
-    int b = t;
-    if (a.q_indptr) {
-        int lo = 0, hi = a.B;
-        while (lo < hi) {
-            const int mid = (lo + hi) / 2;
-            if (a.q_indptr[mid + 1] > t) hi = mid;
-            else lo = mid + 1;
-        }
-        b = lo;
+// A block's operands from the wave's slot, as dec_read_block (of which they are the halves).
+__device__ __forceinline__ void tree_read_k(DecBlock& b, uint8_t* slot, int l16, int lg) {
+    typedef __attribute__((address_space(3))) uint8_t lds_u8;
+    const uint32_t kl = tree_fresh((uint32_t)(l16 * 256 + ((((l16 >> 2) << 2) | (lg ^ (l16 & 3))) << 4)));
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks)
+            b.k[t][ks] = __builtin_bit_cast(pf16x8, *(const __attribute__((address_space(3))) pu32x4*)(
+                                                        (lds_u8*)slot + ((kl ^ (uint32_t)(ks << 6)) + kDecPageBytes * t)));
+}
+__device__ __forceinline__ void tree_read_v(DecBlock& b, uint8_t* slot, int l16, int lg) {
+    typedef __attribute__((address_space(3))) uint8_t lds_u8;
+    const int key = 4 * lg + (l16 >> 2);
+    const uint32_t vl = tree_fresh((uint32_t)(2 * kDecPageBytes + key * 256 + ((((key & 7) << 1) | ((l16 & 3) >> 1)) << 4) + 8 * (l16 & 1)));
+#pragma unroll
+    for (int dt = 0; dt < 8; ++dt) {
+        pf16x4 half[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            half[h] = __builtin_bit_cast(pf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16(
+                (__attribute__((address_space(3))) lds_f16x4*)((lds_u8*)slot + ((vl ^ (uint32_t)(dt << 5)) + kDecPageBytes * h))));
+        b.v[dt] = pf16x8{half[0][0], half[0][1], half[0][2], half[0][3], half[1][0], half[1][1], half[1][2], half[1][3]};
     }
-    if (!live || b >= a.B) return;   // (no barrier below: a wave keeps to its own LDS)
-    const int q0 = a.q_indptr ? a.q_indptr[b] : b, n = a.q_indptr ? a.q_indptr[b + 1] - q0 : 1, i = t - q0;
-    if (i < 0) return;
-    const int pb = a.kv_indptr[b], np = a.kv_indptr[b + 1] - pb;
-    const int len = np > 0 ? (np - 1) * kPage + min(kPage, max(1, a.kv_last[b])) : 0, ctx = len - n;
-    const int pos_q = a.depth ? max(0, a.depth[t]) : i;   // relative to ctx, as below
-    const float slope = a.slopes ? a.slopes[h] * 1.4426950408889634f : 0.f;
-    const _Float16* q = a.q + ((size_t)t * a.Hq + h) * kHeadDim;
-    s_q[wave][lane] = (float)q[lane];
-    s_q[wave][lane + 64] = (float)q[lane + 64];
-    __builtin_amdgcn_wave_barrier();
-    float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
-    for (int base = 0; base < len; base += 64) {
-        const int key = base + lane, j = key - ctx;
-        bool seen = key < len;
-        int pos_k = j;
-        if (seen && j >= 0) {
-            if (a.mask || a.depth) seen = j < kTreeMaxTokens;
-            if (seen) seen = a.mask ? j < 32 * a.mask_words && (a.mask[(size_t)t * a.mask_words + j / 32] >> (j & 31) & 1) : j <= i;
-            if (seen && a.depth) pos_k = max(0, a.depth[q0 + j]);
+}
+
+struct TreePiece {
+    TreeSeq q;
+    int pb, q0;            // first page-table entry and first token (row of q) of the sequence
+    int i0, tokens, rows;  // the group's first token within the sequence, its tokens and rows
+    int p0, p1;            // attended pages of the piece
+    int slot;              // partial slot, or -1
+};
+
+// (so that sums of positions fit an int)
+__device__ __forceinline__ int tree_depth(int d) { return min(max(d, 0), 1 << 28); }
+
+// Position of drafted token j relative to the context, as a key.
+template <int NT>
+__device__ __forceinline__ int tree_key_pos(bool depth, const TreeShared<NT>& S, int j) {
+    return depth && j >= 0 ? S.depth[min(j, kTreeMaxTokens - 1)] : j;
+}
+
+// A piece row by row, for one thing alone: V of a key that some rows see and others do not holds NaN or infinity, which
+// a product with the weight 0 of those others would pass on. A wave per row, 64 keys at a time: a key per lane for
+// the scores, then two dims per lane, over the keys that the row sees.
+template <int NT, bool MOD>
+__device__ __forceinline__ void tree_piece_rows(TreeShared<NT>& S, const TreePiece& p, int kvh, int end) {
+    constexpr int ROWS = 16 * NT;
+    const auto& a = *tree_args();
+    const int wave = __builtin_amdgcn_readfirstlane(tree_fresh(threadIdx.x) >> 6), lane = (int)(tree_fresh(threadIdx.x) & 63u);
+    const TreeSeq& sq = p.q;
+    float* const sp = reinterpret_cast<float*>(S.slot[wave]);             // the weights of 64 keys, then their rows' places
+    int* const spg = reinterpret_cast<int*>(S.slot[wave]) + 64;
+    __syncthreads();   // the waves' outputs in the slots are given up
+    for (int r = wave; r < p.rows; r += kTreeWaves) {
+        const int i = r / a.G, h = kvh * a.G + (r - i * a.G);
+        const size_t row = (size_t)(p.q0 + p.i0 + i) * a.Hq + h;
+        const _Float16* q = a.q + row * kHeadDim;
+        const int pos = MOD && a.depth ? tree_depth(a.depth[p.q0 + p.i0 + i]) : p.i0 + i;
+        const float slope = MOD && a.slopes ? a.slopes[h] * kTreeLog2e : 0.f;
+        float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
+        for (int at = p.p0; at < p.p1; at += 4) {   // four pages
+            const int mine = at + (lane >> 4), page = sq.page(min(mine, p.p1 - 1)), key = page * kPage + (lane & 15), j = key - sq.ctx;
+            bool seen = mine < p.p1 && key < end;
+            if (seen && j >= 0) seen = a.mask ? (S.mask[i][min(j, kTreeMaxTokens - 1) >> 5] >> (j & 31) & 1u) != 0u : j <= p.i0 + i;
+            const int apart = pos - (MOD ? tree_key_pos(a.depth != nullptr, S, j) : j);
+            if (MOD && a.window > 0) seen = seen && (apart < a.window || key < a.sink);
+            const int id = a.kv_indices[p.pb + page];
+            float x = -INFINITY;
+            if (seen) {
+                const size_t off = ((size_t)(uint32_t)id * kPage + (key & 15)) * a.Hkv + kvh;
+                const _Float16* k = reinterpret_cast<const _Float16*>(a.k) + off * kHeadDim;
+                x = 0.f;
+                for (int d = 0; d < kHeadDim; ++d) x = fmaf((float)q[d], (float)k[d], x);
+                if (MOD && a.cap_out > 0.f) {
+                    x *= a.cap_in;
+                    x = a.cap_out * (fabsf(x) <= 1.f ? tree_tanh_small(x) : tree_tanh_large(x));
+                } else {
+                    x *= a.scale_log2;
+                }
+                if (MOD && a.slopes) x = fmaf(slope, (float)-apart, x);
+            }
+            float mx = x;
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) mx = fmaxf(mx, __shfl_xor(mx, d, 64));
+            const float mn = fmaxf(m, mx), al = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+            const float w = seen ? __builtin_amdgcn_exp2f(x - (mn == -INFINITY ? 0.f : mn)) : 0.f;
+            if (m != -INFINITY) {   // (0 times what a row has summed of infinities would be NaN)
+                l *= al;
+                o0 *= al;
+                o1 *= al;
+            }
+            m = mn;
+            l += w;
+            sp[lane] = w;
+            spg[lane] = id;
+            uint64_t todo = __builtin_amdgcn_ballot_w64(seen);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            while (todo) {
+                const int e = __builtin_ctzll(todo);
+                todo &= todo - 1;
+                const size_t off = ((size_t)(uint32_t)spg[e] * kPage + (e & 15)) * a.Hkv + kvh;
+                const _Float16* v = reinterpret_cast<const _Float16*>(a.v) + off * kHeadDim + 2 * lane;
+                o0 = fmaf(sp[e], (float)v[0], o0);
+                o1 = fmaf(sp[e], (float)v[1], o1);
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         }
-        if (a.window > 0 && seen) seen = pos_q - pos_k < a.window || key < a.sink;
-        float x = -INFINITY;
-        if (seen) {
-            const size_t off = ((size_t)(uint32_t)a.kv_indices[pb + key / kPage] * kPage + key % kPage) * a.Hkv + kvh;
-            const _Float16* k = reinterpret_cast<const _Float16*>(a.k) + off * kHeadDim;
-            float dot = 0.f;
-            for (int d = 0; d < kHeadDim; ++d) dot = fmaf(s_q[wave][d], (float)k[d], dot);
-            x = a.cap_out > 0.f ? a.cap_out * tree_tanh(dot * a.cap_in) : dot * a.scale_log2;
-            if (a.slopes) x = fmaf(slope, (float)(pos_k - pos_q), x);
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) l += __shfl_xor(l, d, 64);
+        const float inv = l == 0.f ? 0.f : 1.f / l, lse = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kTreeLn2;
+        if (p.slot < 0) {
+            a.out[row * kHeadDim + 2 * lane] = (_Float16)(o0 * inv);
+            a.out[row * kHeadDim + 2 * lane + 1] = (_Float16)(o1 * inv);
+            if (lane == 0) a.lse[row] = lse;
+        } else {
+            const size_t pr = (size_t)p.slot * ROWS + r;
+            *reinterpret_cast<float2*>(a.part_o + pr * kHeadDim + 2 * lane) = make_float2(o0 * inv, o1 * inv);
+            if (lane == 0) a.part_lse[pr] = lse;
         }
-        const float mn = fmaxf(m, tree_wave_reduce<true>(x));
-        const float al = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
-        const float p = seen ? __builtin_amdgcn_exp2f(x - (mn == -INFINITY ? 0.f : mn)) : 0.f;
-        m = mn;
-        l = l * al + p;
-        o0 *= al;
-        o1 *= al;
-        s_p[wave][lane] = p;
-        s_off[wave][lane] = seen;
-        __builtin_amdgcn_wave_barrier();
-        for (int e = 0; e < 64; ++e) {
-            if (!__builtin_amdgcn_readfirstlane(s_off[wave][e])) continue;
-            const int k2 = base + e;
-            const size_t off = ((size_t)(uint32_t)a.kv_indices[pb + k2 / kPage] * kPage + k2 % kPage) * a.Hkv + kvh;
-            const _Float16* v = reinterpret_cast<const _Float16*>(a.v) + off * kHeadDim + 2 * lane;
-            o0 = fmaf(s_p[wave][e], (float)v[0], o0);
-            o1 = fmaf(s_p[wave][e], (float)v[1], o1);
-        }
-        __builtin_amdgcn_wave_barrier();
     }
-    const float L = tree_wave_reduce<false>(l);
-    const float inv = L == 0.f ? 0.f : 1.f / L;
-    _Float16* out = a.out + ((size_t)t * a.Hq + h) * kHeadDim + 2 * lane;
-    out[0] = (_Float16)(o0 * inv);
-    out[1] = (_Float16)(o1 * inv);
-    if (lane == 0)
-        a.lse[(size_t)t * a.Hq + h] = L == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(L)) * kTreeLn2;
+}
+
+template <int NT, bool MOD>
+__device__ __forceinline__ void tree_piece(TreeShared<NT>& S, const TreePiece& p, int kvh) {
+    constexpr int ROWS = 16 * NT;
+    const auto& a = *tree_args();
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    const int l16 = lane & 15, lg = lane >> 4, G = a.G;
+    const TreeSeq& sq = p.q;
+    const int ctx = sq.ctx;
+
+    __syncthreads();   // the piece before is done with the LDS
+    if (tid == 0) S.wild = 0;
+    if (a.mask) {
+        for (int i = tid; i < p.tokens * kTreeMaskWords; i += kTreeThreads) {
+            const int r = i / kTreeMaskWords, w = i % kTreeMaskWords;
+            S.mask[r][w] = w < a.mask_words ? a.mask[(size_t)(p.q0 + p.i0 + r) * a.mask_words + w] : 0u;
+        }
+    }
+    if (MOD && a.depth)
+        for (int j = tid; j < min(sq.n, kTreeMaxTokens); j += kTreeThreads) S.depth[j] = tree_depth(a.depth[p.q0 + j]);
+
+    // This lane's row of each tile: token i0 + r / G, head kvh G + r % G (rows past the group repeat its last)
+    pf16x8 q[NT][4];
+    int pos[NT];   // the token's position relative to the context
+    float slope[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const int r = min(16 * t + l16, p.rows - 1);
+        const int i = r / G, h = kvh * G + (r - i * G);
+        const size_t row = (size_t)(p.q0 + p.i0 + i) * a.Hq + h;
+        const _Float16* qp = a.q + row * kHeadDim + 8 * lg;
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) q[t][ks] = *reinterpret_cast<const pf16x8*>(qp + 32 * ks);
+        pos[t] = MOD && a.depth ? tree_depth(a.depth[p.q0 + p.i0 + i]) : p.i0 + i;
+        slope[t] = MOD && a.slopes ? a.slopes[h] * kTreeLog2e : 0.f;
+        if (!MOD) dec_sign_q(q[t], a.scale_log2);
+    }
+    // Keys every row sees: [full_lo, full_hi), and those below full_sink. Keys no row sees: from end on.
+    const bool tree = a.mask || a.depth;
+    const int full_hi = tree ? ctx : ctx + p.i0 + 1;
+    int end = a.mask ? sq.len : min(sq.len, ctx + p.i0 + p.tokens);
+    if (tree) end = min(end, ctx + kTreeMaxTokens);
+    int full_lo = 0, full_sink = 0;
+    if (MOD && a.window > 0) {
+        int mx = pos[0];
+#pragma unroll
+        for (int t = 1; t < NT; ++t) mx = max(mx, pos[t]);
+#pragma unroll
+        for (int d = 1; d < 16; d <<= 1) mx = max(mx, __shfl_xor(mx, d, 64));
+        full_lo = __builtin_amdgcn_readfirstlane(max(0, ctx + mx - a.window + 1));
+        full_sink = a.sink;
+    }
+    // Of the piece's pages those that hold a key some row sees. (The attended places ascend with the page.)
+    const int np_end = max(0, (end + kPage - 1) / kPage);   // pages [0, np_end)
+    const int att_end = np_end <= sq.s ? np_end : np_end <= sq.w0 ? sq.s : sq.s + np_end - sq.w0;
+    const int p1 = min(p.p1, att_end);
+    const int npg = p1 - p.p0;
+    // this wave's blocks: attended places p0 + 8 i + 2 wave and the next
+    const int nblk = npg > 2 * wave ? (npg - 2 * wave + 7) / 8 : 0;
+
+    const uint32_t page_bytes = (uint32_t)(kPage * a.Hkv * 256);
+    // Row n = 4 i + lg of a page, LDS position l16 of it: chunk l16 ^ n of K, l16 ^ ((n & 7) << 1) of V (the swizzles that
+    // dec_read_block reads): from the bases of row lg, ^ i << 6 and ^ (i & 1) << 7, + i rows4.
+    const uint32_t kbase = (uint32_t)(lg * a.Hkv * 256 + ((l16 ^ lg) << 4)), vbase = (uint32_t)(lg * a.Hkv * 256 + ((l16 ^ (lg << 1)) << 4));
+    const uint32_t rows4 = (uint32_t)(4 * a.Hkv * 256);
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)S.slot[wave];
+    const uint8_t* const kc = a.k + kvh * 256;
+    const uint8_t* const vc = a.v + kvh * 256;
+    // lane 2 x + y holds page y of block x of a window of 32 blocks
+    int pidv = 0;
+    auto load_ids = [&](int blk) {
+        const int at = p.p0 + 8 * (blk + (lane >> 1)) + 2 * wave + (lane & 1);
+        pidv = a.kv_indices[p.pb + sq.page(min(at, p1 - 1))];
+    };
+    auto issue = [&](int blk) {
+        if (blk >= nblk) return;
+        const int at = p.p0 + 8 * blk + 2 * wave;
+        const uint32_t kb = tree_fresh(kbase), vb = tree_fresh(vbase);
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+            if (at + y >= p1) break;
+            const size_t off = (size_t)(uint32_t)__builtin_amdgcn_readlane(pidv, 2 * (blk & 31) + y) * page_bytes;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) dec_dma(kc + off, (kb ^ (uint32_t)(i << 6)) + i * rows4, lds0 + kDecPageBytes * y + 1024 * i);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) dec_dma(vc + off, (vb ^ (uint32_t)((i & 1) << 7)) + i * rows4, lds0 + kDecPageBytes * (2 + y) + 1024 * i);
+        }
+    };
+
+    uint32_t wild = 0u;   // not 0: an element of V, of a key that not every row may see, is not finite
+    float m[NT], l[NT];
+    pf32x4 acc[NT][8];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        m[t] = -INFINITY;
+        l[t] = 0.f;
+#pragma unroll
+        for (int dt = 0; dt < 8; ++dt) acc[t][dt] = pf32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    // (a scale of 0 would make an unseen key's -inf a NaN)
+    const float scale2 = MOD ? 1.f : a.scale_log2 == 0.f ? 0x1p-126f : fabsf(a.scale_log2);
+
+    __syncthreads();   // mask rows and depths
+    if (nblk > 0) {
+        load_ids(0);
+        issue(0);
+    }
+    for (int blk = 0; blk < nblk; ++blk) {
+        // One tile: all operands to registers, and the next block's loads are on their way before any arithmetic. Two
+        // tiles: K first, V after the scores, in the registers of K.
+        DecBlock b;
+        dec_wait_loads();
+        tree_read_k(b, S.slot[wave], l16, lg);
+        if constexpr (NT == 1) tree_read_v(b, S.slot[wave], l16, lg);
+        dec_wait_lds();
+        auto next = [&]() {
+            if (((blk + 1) & 31) == 0 && blk + 1 < nblk) load_ids(blk + 1);
+            issue(blk + 1);
+        };
+        if constexpr (NT == 1) next();
+
+        const int at = p.p0 + 8 * blk + 2 * wave;
+        const bool two = at + 1 < p1;
+        const int tok0 = sq.page(at) * kPage, tok1 = two ? sq.page(at + 1) * kPage : end;
+        float x[NT][8];
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+                pf32x4 c0 = pf32x4{0.f, 0.f, 0.f, 0.f}, c1 = c0;
+                c0 = mfma16x16x32(b.k[y][0], q[t][0], c0);
+                c1 = mfma16x16x32(b.k[y][1], q[t][1], c1);
+                c0 = mfma16x16x32(b.k[y][2], q[t][2], c0);
+                c1 = mfma16x16x32(b.k[y][3], q[t][3], c1);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[t][4 * y + j] = c0[j] + c1[j];
+            }
+        if constexpr (NT > 1) {
+            __builtin_amdgcn_sched_barrier(0);
+            tree_read_v(b, S.slot[wave], l16, lg);
+            dec_wait_lds();
+            next();
+        }
+        bool biased = false;
+        if constexpr (MOD) {
+            const auto& h = *tree_args();
+            const float cap_in = h.cap_in, cap_out = h.cap_out, scale_log2 = h.scale_log2;
+            biased = h.slopes != nullptr;
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                if (cap_out > 0.f) {   // (uniform)
+                    float top = 0.f;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        x[t][e] *= cap_in;
+                        top = fmaxf(top, fabsf(x[t][e]));
+                    }
+                    if (__builtin_amdgcn_ballot_w64(!(top <= 1.f))) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const float s = tree_tanh_small(x[t][e]), g = tree_tanh_large(x[t][e]);
+                            x[t][e] = cap_out * (fabsf(x[t][e]) <= 1.f ? s : g);
+                            __builtin_amdgcn_sched_barrier(0);
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) x[t][e] = cap_out * tree_tanh_small(x[t][e]);
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[t][e] *= scale_log2;
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        // Which of the lane's 8 keys each of its rows sees (bits); all, in a block inside every row's keys.
+        auto inside = [&](int tk) { return tk + kPage <= full_hi && (tk >= full_lo || tk + kPage <= full_sink); };
+        const bool plain = two && inside(tok0) && inside(tok1);   // (uniform)
+        if (plain) {
+            if (biased) {
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const int key = (e < 4 ? tok0 : tok1) + 4 * lg + (e & 3);
+                        x[t][e] = fmaf(slope[t], (float)(key - ctx - pos[t]), x[t][e]);
+                    }
+            }
+        } else {
+            // (bits by integer arithmetic: conditions would fill the scalar registers)
+            const auto& f = *tree_args();
+            auto below = [](int n) { return (1u << min(max(n, 0), 4)) - 1u; };   // the first n of 4 keys
+            const int gs = __builtin_ctz(f.G);   // G is a power of two
+            const int lg4 = (int)(tree_fresh(lane) >> 4) * 4, k0 = tok0 + lg4, k1 = tok1 + lg4;
+            const uint32_t real = below(end - k0) | below(two ? end - k1 : 0) << 4;
+            uint32_t near[NT];   // inside the window
+#pragma unroll
+            for (int t = 0; t < NT; ++t) near[t] = 0xFFu;
+            if constexpr (MOD) {
+                const int window = f.window;
+                const uint32_t kept = below(f.sink - k0) | below(f.sink - k1) << 4;
+                if (window > 0) {
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) near[t] = kept;
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int at_key = tree_key_pos(f.depth != nullptr, S, (e < 4 ? k0 : k1) + (e & 3) - ctx);
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) {
+                        const int apart = pos[t] - at_key;
+                        near[t] |= (uint32_t)(apart - window) >> 31 << e;
+                        if (biased) x[t][e] = fmaf(slope[t], (float)-apart, x[t][e]);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+            uint32_t seen[NT];
+            if (f.mask) {
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    const int tok = min(16 * t + (int)(tree_fresh(lane) & 15u), p.rows - 1) >> gs;
+                    // 4 bits from drafted token j on; those before the first are cached keys, seen
+                    auto bits = [&](int j) {
+                        const int w = j >> 5;
+                        const uint32_t* row = S.mask[tok];
+                        const uint32_t lo = w < 0 ? ~0u : row[min(w, kTreeMaskWords - 1)];
+                        const uint32_t hi = w < -1 ? ~0u : w + 1 < kTreeMaskWords ? row[w + 1] : 0u;
+                        return __builtin_amdgcn_alignbit(hi, lo, (uint32_t)j & 31u) & 15u;
+                    };
+                    seen[t] = real & near[t] & (bits(k0 - ctx) | bits(k1 - ctx) << 4);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            } else {
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    const int upto = ctx + p.i0 + (min(16 * t + (int)(tree_fresh(lane) & 15u), p.rows - 1) >> gs) + 1;
+                    seen[t] = real & near[t] & (below(upto - k0) | below(upto - k1) << 4);
+                }
+            }
+            uint32_t keep[4];   // the V elements of real keys
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                keep[i] = ((uint32_t)((int)(real << (31 - 2 * i)) >> 31) & 0xFFFFu) | ((uint32_t)((int)(real << (30 - 2 * i)) >> 31) & 0xFFFF0000u);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[t][e] = seen[t] >> e & 1u ? x[t][e] : -INFINITY;
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            uint32_t odd = 0u;
+#pragma unroll
+            for (int dt = 0; dt < 8; ++dt) {
+                pu32x4 w = __builtin_bit_cast(pu32x4, b.v[dt]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    w[i] &= keep[i];
+                    odd |= ((w[i] & 0x7C00u) == 0x7C00u) | ((w[i] & 0x7C000000u) == 0x7C000000u);
+                }
+                b.v[dt] = __builtin_bit_cast(pf16x8, w);
+            }
+            wild |= odd;
+        }
+
+        // Online softmax in base 2. The weights carry a factor 2^15, in l and in the PV product alike, so that fp16
+        // holds them down to 2^-39 of the running maximum's.
+        float mn[NT];
+        bool grow = false;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            float mx = x[t][0];
+#pragma unroll
+            for (int e = 1; e < 8; ++e) mx = fmaxf(mx, x[t][e]);
+            mn[t] = fmaxf(m[t], col4_reduce<true>(mx));
+            grow |= mn[t] > m[t];
+        }
+        if (__builtin_amdgcn_ballot_w64(grow)) {
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                const float al = mn[t] > m[t] ? __builtin_amdgcn_exp2f((m[t] - mn[t]) * scale2) : 1.f;
+                l[t] *= al;
+#pragma unroll
+                for (int dt = 0; dt < 8; ++dt) acc[t][dt] *= al;
+                m[t] = mn[t];
+            }
+        }
+        pf16x8 w[NT];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const float ms = m[t] == -INFINITY ? 0.f : m[t];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float pe = __builtin_amdgcn_exp2f(fmaf(x[t][e] - ms, scale2, 15.f));
+                l[t] += pe;
+                w[t][e] = (_Float16)pe;
+            }
+        }
+#pragma unroll
+        for (int dt = 0; dt < 8; ++dt)
+#pragma unroll
+            for (int t = 0; t < NT; ++t) acc[t][dt] = mfma16x16x32(b.v[dt], w[t], acc[t][dt]);
+    }
+
+    // Join of the four waves: each leaves its output in its slot (row r's four dims c at place c ^ r of the row, so
+    // that the 16 rows of a store lie in different banks).
+    dec_wait_lds();
+    if (__builtin_amdgcn_ballot_w64(wild != 0u) && lane == 0) S.wild = 1;
+    float* const so = reinterpret_cast<float*>(S.slot[wave]);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const float L = col4_reduce<false>(l[t]);
+        if (lg == 0) {
+            S.m[wave][16 * t + l16] = m[t];
+            S.l[wave][16 * t + l16] = L;
+        }
+#pragma unroll
+        for (int dt = 0; dt < 8; ++dt)
+            *reinterpret_cast<pf32x4*>(so + ((16 * t + l16) * 32 + ((4 * dt + lg) ^ l16)) * 4) = acc[t][dt];
+    }
+    __syncthreads();
+    const auto& f = *tree_args();
+    const int kvh_ = (int)tree_fresh_s(blockIdx.x) % f.Hkv;
+    if (S.wild) {   // (uniform)
+        tree_piece_rows<NT, MOD>(S, p, kvh_, end);
+        return;
+    }
+#pragma unroll 1
+    for (int it = 0; it < ROWS * 32 / kTreeThreads; ++it) {
+        const int idx = it * kTreeThreads + (int)tree_fresh(threadIdx.x), r = idx >> 5, c = idx & 31;
+        if (r >= p.rows) continue;
+        float mw[kTreeWaves], M = -INFINITY, L = 0.f;
+        pf32x4 o = pf32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < kTreeWaves; ++w) {
+            mw[w] = S.m[w][r];
+            M = fmaxf(M, mw[w]);
+        }
+#pragma unroll
+        for (int w = 0; w < kTreeWaves; ++w) {
+            const float al = mw[w] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((mw[w] - M) * scale2);
+            const pf32x4 v = *reinterpret_cast<const pf32x4*>(reinterpret_cast<const float*>(S.slot[w]) + (r * 32 + (c ^ (r & 15))) * 4);
+            L = fmaf(al, S.l[w][r], L);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[j] = fmaf(al, v[j], o[j]);
+        }
+        const float inv = L == 0.f ? 0.f : 1.f / L;
+        const float lse = L == 0.f ? -INFINITY : fmaf(M, scale2, __builtin_amdgcn_logf(L) - 15.f) * kTreeLn2;
+        if (p.slot < 0) {
+            const int i = r / f.G;
+            const size_t row = (size_t)(p.q0 + p.i0 + i) * f.Hq + kvh_ * f.G + (r - i * f.G);
+            const pf16x4 h = {(_Float16)(o[0] * inv), (_Float16)(o[1] * inv), (_Float16)(o[2] * inv), (_Float16)(o[3] * inv)};
+            *reinterpret_cast<pf16x4*>(f.out + row * kHeadDim + 4 * c) = h;
+            if (c == 0) f.lse[row] = lse;
+        } else {
+            const size_t row = (size_t)p.slot * ROWS + r;
+            *reinterpret_cast<pf32x4*>(f.part_o + row * kHeadDim + 4 * c) = o * inv;
+            if (c == 0) f.part_lse[row] = lse;
+        }
+    }
+}
+
+template <int NT, bool MOD>
+__global__ __launch_bounds__(kTreeThreads, 2) void tree_split_kernel(TreeArgs a) {
+    __shared__ TreeShared<NT> S;
+    const int g = blockIdx.x / a.Hkv, kvh = blockIdx.x - g * a.Hkv;
+    int64_t lo, hi, units;
+    int ranges;
+    const bool some = tree_find_range(a, S.scan, g, lo, hi, units, ranges);
+    if (!some) {
+        if (kvh == 0 && threadIdx.x == 0) a.cuts[g] = make_int4(0, 0, 0, 0);
+        return;
+    }
+    // The first item, the units of it before the range, and (kv head 0) what the merge has to know: an item that
+    // the boundary before this range is the first to cut, and its pieces.
+    int b = __builtin_amdgcn_readfirstlane(S.scan.first), j, skip;
+    int left = (int)(hi - lo);
+    {
+        const auto& k = *tree_args();
+        int q0, pb;
+        const TreeSeq t = tree_load_seq(k, b, &q0, &pb);
+        const int64_t in = lo - S.scan.prefix;
+        j = (int)(in / t.units());
+        skip = (int)(in - (int64_t)j * t.units());
+        if (kvh == 0 && threadIdx.x == 0) {
+            const int64_t first = lo - skip;
+            const int g0 = tree_range_of(units, ranges, first), g1 = tree_range_of(units, ranges, first + t.units() - 1);
+            const int i0 = j * k.tpg;
+            k.cuts[g] = make_int4(q0 + i0, min(k.tpg, t.n - i0) * k.G, skip > 0 && g0 == g - 1 ? g1 - g0 + 1 : 0, 0);
+        }
+    }
+    while (left > 0) {
+        TreePiece p;
+        const auto& k = *tree_args();
+        if (b >= k.B) break;   // (not reached: the units of the items from here on are at least `left`)
+        p.q = tree_load_seq(k, b, &p.q0, &p.pb);
+        if (j >= p.q.groups) {
+            ++b;
+            j = 0;
+            continue;
+        }
+        const int take = min(left, p.q.units() - skip);
+        p.i0 = j * k.tpg;
+        p.tokens = min(k.tpg, p.q.n - p.i0);
+        p.rows = p.tokens * k.G;
+        p.p0 = skip;
+        p.p1 = min(skip + take, p.q.attended());
+        const int s = tree_slot(skip, take, p.q.units());
+        p.slot = s < 0 ? -1 : 2 * (int)blockIdx.x + s;
+        left -= take;
+        skip = 0;
+        ++j;
+        tree_piece<NT, MOD>(S, p, kvh);
+    }
+}
+
+// Merge of the cut items: boundary g, kv head, four rows a workgroup, a row per wave. Each half of a wave takes every
+// second piece, four dims a lane, in order; the halves are joined at the end (a fixed order).
+__global__ __launch_bounds__(kTreeThreads) void tree_merge_kernel(TreeArgs a, int ROWS) {
+    const int g = blockIdx.x / a.Hkv + 1, kvh = blockIdx.x % a.Hkv;
+    const int4 cut = a.cuts[g];
+    const int n = cut.z;
+    if (n == 0) return;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, half = lane >> 5, c = lane & 31;
+    for (int r = blockIdx.y * kTreeWaves + wave; r < cut.y; r += gridDim.y * kTreeWaves) {
+        // piece k: range g - 1 + k, slot 1 of the first's workgroup, slot 0 of the others'
+        auto slot = [&](int k) { return ((size_t)((g - 1 + k) * a.Hkv + kvh) * 2 + (k == 0)) * ROWS + r; };
+        float m = -INFINITY, ws = 0.f;
+        pf32x4 o = pf32x4{0.f, 0.f, 0.f, 0.f};
+        constexpr int U = 4;
+        for (int k0 = half; k0 - half < n; k0 += 2 * U) {
+            float l[U];
+            pf32x4 v[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const size_t s = slot(min(k0 + 2 * u, n - 1));
+                l[u] = a.part_lse[s];
+                v[u] = *reinterpret_cast<const pf32x4*>(a.part_o + s * kHeadDim + 4 * c);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (k0 + 2 * u >= n || l[u] == -INFINITY) continue;
+                const float mn = fmaxf(m, l[u]);
+                const float sc = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - mn) * kTreeLog2e);
+                const float w = __builtin_amdgcn_exp2f((l[u] - mn) * kTreeLog2e);
+                ws = fmaf(ws, sc, w);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) o[j] = fmaf(w, v[u][j], o[j] * sc);
+                m = mn;
+            }
+        }
+        const float m2 = __shfl_xor(m, 32, 64), ws2 = __shfl_xor(ws, 32, 64), M = fmaxf(m, m2);
+        const float s1 = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - M) * kTreeLog2e);
+        const float s2 = m2 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m2 - M) * kTreeLog2e);
+        // (the lower half's pieces first, in both)
+        const float W = half == 0 ? ws * s1 + ws2 * s2 : ws2 * s2 + ws * s1;
+        const float inv = W == 0.f ? 0.f : 1.f / W;
+        pf16x4 h;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float o2 = __shfl_xor(o[j], 32, 64);
+            h[j] = (_Float16)((o[j] * s1 + o2 * s2) * inv);
+        }
+        if (half == 0) {
+            const int i = r / a.G;
+            const size_t row = (size_t)(cut.x + i) * a.Hq + kvh * a.G + (r - i * a.G);
+            *reinterpret_cast<pf16x4*>(a.out + row * kHeadDim + 4 * c) = h;
+            if (c == 0) a.lse[row] = W == 0.f ? -INFINITY : m == -INFINITY && m2 == -INFINITY ? W : M + __builtin_amdgcn_logf(W) * kTreeLn2;
+        }
+    }
+}
+
+template <int NT>
+void launch_tree_split(const TreeArgs& a, bool mod, hipStream_t s) {
+    const int W = a.ranges * a.Hkv;
+    if (mod) tree_split_kernel<NT, true><<<W, kTreeThreads, 0, s>>>(a);
+    else tree_split_kernel<NT, false><<<W, kTreeThreads, 0, s>>>(a);
 }
 
 }  // namespace
 
 hipError_t launch_tree_attention(const TreeArgs& a, hipStream_t s) {
-    const int64_t rows = (int64_t)a.n_tokens * a.Hq;
-    if (rows <= 0 || a.B <= 0) return hipSuccess;
-    tree_rows_kernel<<<(unsigned)((rows + kTreeWaves - 1) / kTreeWaves), kTreeWaves * 64, 0, s>>>(a);
+    if (a.n_tokens <= 0 || a.B <= 0 || a.ranges <= 0) return hipSuccess;
+    const bool mod = a.cap_out > 0.f || a.slopes || a.window > 0;
+    if (a.rows == 16) launch_tree_split<1>(a, mod, s);
+    else if (a.rows == 32) launch_tree_split<2>(a, mod, s);
+    else return hipErrorInvalidValue;
+    if (a.ranges > 1) {
+        const int most = std::min(a.rows, std::max(1, a.max_tokens) * a.G);
+        tree_merge_kernel<<<dim3((a.ranges - 1) * a.Hkv, (most + kTreeWaves - 1) / kTreeWaves), kTreeThreads, 0, s>>>(a, a.rows);
+    }
     return hipGetLastError();
 }
 

@@ -437,7 +437,7 @@ typedef struct pdattn_score_params {
  *     for a tree, its ancestors and itself;
  *   - without a mask, if j <= i (a chain).
  * Positions, for slopes and window: key t < ctx_b is at t, token i (as a query and as a key) at
- * ctx_b + depth[i], or ctx_b + i without depth; a depth below 0 counts as 0.
+ * ctx_b + depth[i], or ctx_b + i without depth; depths count as at least 0 and at most 2^28.
  * A token that sees no key gets out = 0, lse = -inf. Keys that a token does not see have no influence
  * on it, whatever bits they hold. Rows of q, out and lse from q_indptr[B] on are neither read nor written.
  * Nothing on the host depends on the lengths, the trees or q_indptr, so a captured call can be replayed
