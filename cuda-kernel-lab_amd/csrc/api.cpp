@@ -1648,7 +1648,7 @@ int tree_layout(const pdattn_tree_params* p, int G, TreeLayout* L) {
     DeviceFacts f;
     if (int st = device_facts(&f)) return st;
     const int64_t rows = (int64_t)(p->q_indptr ? p->max_tokens : 1) * G;
-    L->rows = rows <= 16 ? 16 : 32;
+    L->rows = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
     L->ranges = std::max(1, 2 * f.cus / p->Hkv);
     const size_t slots = (size_t)2 * L->ranges * p->Hkv * L->rows;
     size_t off = align_up(sizeof(int4) * L->ranges);

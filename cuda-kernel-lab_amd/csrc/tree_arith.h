@@ -53,6 +53,27 @@ PD_RANGE_FN TreeSeq tree_seq(int ip0, int ip1, int last, int q0, int q1, int n_t
     return t;
 }
 
+// The attended pages of a sequence below page `p` (those before it in the order of places).
+PD_RANGE_FN int tree_places_below(const TreeSeq& t, int p) { return p <= t.s ? p : p <= t.w0 ? t.s : t.s + p - t.w0; }
+
+// The blocks of a wave: block i starts at place first + step i and has `width` places, those below p1. Places [a0, a1) hold
+// pages whose every key is seen by every row: the blocks inside them are `plain`, and come first; then those behind
+// them, then those before (the order of blocks does not matter to a softmax, and two loops without a branch inside do).
+struct TreeOrder {
+    int n, b0, plain;
+    PD_RANGE_FN int block(int i) const { return i + b0 < n ? i + b0 : i + b0 - n; }
+};
+PD_RANGE_FN TreeOrder tree_order(int first, int step, int width, int p1, int a0, int a1) {
+    TreeOrder o;
+    o.n = first < p1 ? (p1 - first + step - 1) / step : 0;
+    if (a1 > p1) a1 = p1;
+    o.b0 = a0 > first ? (a0 - first + step - 1) / step : 0;
+    const int b1 = a1 >= first + width ? (a1 - first - width) / step + 1 : 0;
+    o.plain = b1 > o.b0 ? b1 - o.b0 : 0;
+    if (o.plain == 0) o.b0 = 0;
+    return o;
+}
+
 // Ranges that `units` are cut into: at most `most`, of at least `least` units each.
 PD_RANGE_FN int tree_ranges(int64_t units, int most, int least) {
     const int64_t r = units / least;

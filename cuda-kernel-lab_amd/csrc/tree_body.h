@@ -136,18 +136,30 @@ __device__ __forceinline__ bool tree_find_range(const TreeArgs& a, TreeScan& S, 
 
 // ---- one piece ------------------------------------------------------------------------------------
 
-template <int NT>
-struct TreeShared {
-    static constexpr int ROWS = 16 * NT;
-    alignas(256) uint8_t slot[kTreeWaves][kDecSlotBytes];   // a block of the wave's; at the end its output
-    float m[kTreeWaves][ROWS];
-    float l[kTreeWaves][ROWS];
+// What a piece of either body has in LDS.
+template <int ROWS_>
+struct TreeCommon {
+    static constexpr int ROWS = ROWS_;
     uint32_t mask[ROWS][kTreeMaskWords];                    // the group's mask rows
     int depth[kTreeMaxTokens];                              // the sequence's drafted tokens' depths
     TreeScan scan;
     int wild;                                               // the piece goes row by row (tree_piece_rows)
 };
-static_assert(TreeShared<2>::ROWS * kHeadDim * 4 <= kDecSlotBytes, "a wave's output fits its slot");
+// The key-split body: 16 NT rows, every wave all of them.
+template <int NT>
+struct TreeSplitShared : TreeCommon<16 * NT> {
+    alignas(256) uint8_t slot[kTreeWaves][kDecSlotBytes];   // a block of the wave's; at the end its output
+    float m[kTreeWaves][16 * NT];
+    float l[kTreeWaves][16 * NT];
+    __device__ __forceinline__ uint8_t* scratch(int wave) { return slot[wave]; }
+};
+static_assert(16 * 2 * kHeadDim * 4 <= kDecSlotBytes, "a wave's output fits its slot");
+// The row-split body: 64 NT rows, 16 NT of them each wave's, and 64-key blocks that all waves read.
+template <int NT>
+struct TreeWideShared : TreeCommon<64 * NT> {
+    alignas(256) uint8_t block[2][4 * kDecSlotBytes / 2];   // K of four pages, then V of four pages
+    __device__ __forceinline__ uint8_t* scratch(int wave) { return block[0] + 1024 * wave; }
+};
 
 // The value itself, as a new value in every call: what is formed from it is not kept across the loop.
 __device__ __forceinline__ uint32_t tree_fresh(uint32_t v) {
@@ -198,22 +210,54 @@ struct TreePiece {
 __device__ __forceinline__ int tree_depth(int d) { return min(max(d, 0), 1 << 28); }
 
 // Position of drafted token j relative to the context, as a key.
-template <int NT>
-__device__ __forceinline__ int tree_key_pos(bool depth, const TreeShared<NT>& S, int j) {
+template <class Sh>
+__device__ __forceinline__ int tree_key_pos(bool depth, const Sh& S, int j) {
     return depth && j >= 0 ? S.depth[min(j, kTreeMaxTokens - 1)] : j;
+}
+
+// Which keys a piece's rows see: none from `end` on (so none in places from p1 on), and every row all keys of the pages at
+// places [a0, a1).
+struct TreeKeys {
+    int end, p1, a0, a1;
+};
+template <bool MOD, class A>
+__device__ __forceinline__ TreeKeys tree_keys(const A& a, const TreePiece& p, int lane) {
+    TreeKeys k;
+    const TreeSeq& sq = p.q;
+    const bool tree = a.mask || a.depth;
+    k.end = a.mask ? sq.len : min(sq.len, sq.ctx + p.i0 + p.tokens);
+    if (tree) k.end = min(k.end, sq.ctx + kTreeMaxTokens);
+    k.p1 = min(p.p1, tree_places_below(sq, max(0, (k.end + kPage - 1) / kPage)));
+    // of the keys below `hi` every row sees those from `lo` on: the window's start at the last position of the group
+    const int hi = tree ? sq.ctx : sq.ctx + p.i0 + 1;
+    int lo = 0;
+    if (MOD && a.window > 0) {
+        int last = p.i0 + p.tokens - 1;
+        if (a.depth) {
+            last = 0;
+            for (int i = lane; i < p.tokens; i += 64) last = max(last, tree_depth(a.depth[p.q0 + p.i0 + i]));
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) last = max(last, __shfl_xor(last, d, 64));
+            last = __builtin_amdgcn_readfirstlane(last);
+        }
+        lo = max(0, sq.ctx + last - a.window + 1);
+    }
+    k.a0 = tree_places_below(sq, (lo + kPage - 1) / kPage);
+    k.a1 = tree_places_below(sq, max(0, hi) / kPage);
+    return k;
 }
 
 // A piece row by row, for one thing alone: V of a key that some rows see and others do not holds NaN or infinity, which
 // a product with the weight 0 of those others would pass on. A wave per row, 64 keys at a time: a key per lane for
 // the scores, then two dims per lane, over the keys that the row sees.
-template <int NT, bool MOD>
-__device__ __forceinline__ void tree_piece_rows(TreeShared<NT>& S, const TreePiece& p, int kvh, int end) {
-    constexpr int ROWS = 16 * NT;
+template <bool MOD, class Sh>
+__device__ __forceinline__ void tree_piece_rows(Sh& S, const TreePiece& p, int kvh, int end) {
+    constexpr int ROWS = Sh::ROWS;
     const auto& a = *tree_args();
     const int wave = __builtin_amdgcn_readfirstlane(tree_fresh(threadIdx.x) >> 6), lane = (int)(tree_fresh(threadIdx.x) & 63u);
     const TreeSeq& sq = p.q;
-    float* const sp = reinterpret_cast<float*>(S.slot[wave]);             // the weights of 64 keys, then their rows' places
-    int* const spg = reinterpret_cast<int*>(S.slot[wave]) + 64;
+    float* const sp = reinterpret_cast<float*>(S.scratch(wave));          // the weights of 64 keys, then their pages
+    int* const spg = reinterpret_cast<int*>(S.scratch(wave)) + 64;
     __syncthreads();   // the waves' outputs in the slots are given up
     for (int r = wave; r < p.rows; r += kTreeWaves) {
         const int i = r / a.G, h = kvh * a.G + (r - i * a.G);
@@ -285,7 +329,7 @@ __device__ __forceinline__ void tree_piece_rows(TreeShared<NT>& S, const TreePie
 }
 
 template <int NT, bool MOD>
-__device__ __forceinline__ void tree_piece(TreeShared<NT>& S, const TreePiece& p, int kvh) {
+__device__ __forceinline__ void tree_piece(TreeSplitShared<NT>& S, const TreePiece& p, int kvh) {
     constexpr int ROWS = 16 * NT;
     const auto& a = *tree_args();
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
@@ -320,28 +364,9 @@ __device__ __forceinline__ void tree_piece(TreeShared<NT>& S, const TreePiece& p
         slope[t] = MOD && a.slopes ? a.slopes[h] * kTreeLog2e : 0.f;
         if (!MOD) dec_sign_q(q[t], a.scale_log2);
     }
-    // Keys every row sees: [full_lo, full_hi), and those below full_sink. Keys no row sees: from end on.
-    const bool tree = a.mask || a.depth;
-    const int full_hi = tree ? ctx : ctx + p.i0 + 1;
-    int end = a.mask ? sq.len : min(sq.len, ctx + p.i0 + p.tokens);
-    if (tree) end = min(end, ctx + kTreeMaxTokens);
-    int full_lo = 0, full_sink = 0;
-    if (MOD && a.window > 0) {
-        int mx = pos[0];
-#pragma unroll
-        for (int t = 1; t < NT; ++t) mx = max(mx, pos[t]);
-#pragma unroll
-        for (int d = 1; d < 16; d <<= 1) mx = max(mx, __shfl_xor(mx, d, 64));
-        full_lo = __builtin_amdgcn_readfirstlane(max(0, ctx + mx - a.window + 1));
-        full_sink = a.sink;
-    }
-    // Of the piece's pages those that hold a key some row sees. (The attended places ascend with the page.)
-    const int np_end = max(0, (end + kPage - 1) / kPage);   // pages [0, np_end)
-    const int att_end = np_end <= sq.s ? np_end : np_end <= sq.w0 ? sq.s : sq.s + np_end - sq.w0;
-    const int p1 = min(p.p1, att_end);
-    const int npg = p1 - p.p0;
-    // this wave's blocks: attended places p0 + 8 i + 2 wave and the next
-    const int nblk = npg > 2 * wave ? (npg - 2 * wave + 7) / 8 : 0;
+    const TreeKeys ks = tree_keys<MOD>(a, p, lane);
+    const int end = ks.end, p1 = ks.p1;
+    const TreeOrder o = tree_order(p.p0 + 2 * wave, 8, 2, p1, ks.a0, ks.a1);
 
     const uint32_t page_bytes = (uint32_t)(kPage * a.Hkv * 256);
     // Row n = 4 i + lg of a page, LDS position l16 of it: chunk l16 ^ n of K, l16 ^ ((n & 7) << 1) of V (the swizzles that
@@ -351,20 +376,20 @@ __device__ __forceinline__ void tree_piece(TreeShared<NT>& S, const TreePiece& p
     const uint32_t lds0 = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)S.slot[wave];
     const uint8_t* const kc = a.k + kvh * 256;
     const uint8_t* const vc = a.v + kvh * 256;
-    // lane 2 x + y holds page y of block x of a window of 32 blocks
+    // lane 2 x + y holds page y of the x-th block of a window of 32
     int pidv = 0;
-    auto load_ids = [&](int blk) {
-        const int at = p.p0 + 8 * (blk + (lane >> 1)) + 2 * wave + (lane & 1);
-        pidv = a.kv_indices[p.pb + sq.page(min(at, p1 - 1))];
+    auto load_ids = [&](int i) {
+        const int at = p.p0 + 8 * o.block(min(i + (lane >> 1), o.n - 1)) + 2 * wave + (lane & 1);
+        pidv = tree_args()->kv_indices[p.pb + sq.page(min(at, p1 - 1))];
     };
-    auto issue = [&](int blk) {
-        if (blk >= nblk) return;
-        const int at = p.p0 + 8 * blk + 2 * wave;
+    auto issue = [&](int n) {
+        if (n >= o.n) return;
+        const int at = p.p0 + 8 * o.block(n) + 2 * wave;
         const uint32_t kb = tree_fresh(kbase), vb = tree_fresh(vbase);
 #pragma unroll
         for (int y = 0; y < 2; ++y) {
             if (at + y >= p1) break;
-            const size_t off = (size_t)(uint32_t)__builtin_amdgcn_readlane(pidv, 2 * (blk & 31) + y) * page_bytes;
+            const size_t off = (size_t)(uint32_t)__builtin_amdgcn_readlane(pidv, 2 * (n & 31) + y) * page_bytes;
 #pragma unroll
             for (int i = 0; i < 4; ++i) dec_dma(kc + off, (kb ^ (uint32_t)(i << 6)) + i * rows4, lds0 + kDecPageBytes * y + 1024 * i);
 #pragma unroll
@@ -385,12 +410,8 @@ __device__ __forceinline__ void tree_piece(TreeShared<NT>& S, const TreePiece& p
     // (a scale of 0 would make an unseen key's -inf a NaN)
     const float scale2 = MOD ? 1.f : a.scale_log2 == 0.f ? 0x1p-126f : fabsf(a.scale_log2);
 
-    __syncthreads();   // mask rows and depths
-    if (nblk > 0) {
-        load_ids(0);
-        issue(0);
-    }
-    for (int blk = 0; blk < nblk; ++blk) {
+    auto block = [&](int n, auto EDGE) {
+        constexpr bool edge = decltype(EDGE)::value;
         // One tile: all operands to registers, and the next block's loads are on their way before any arithmetic. Two
         // tiles: K first, V after the scores, in the registers of K.
         DecBlock b;
@@ -399,13 +420,13 @@ __device__ __forceinline__ void tree_piece(TreeShared<NT>& S, const TreePiece& p
         if constexpr (NT == 1) tree_read_v(b, S.slot[wave], l16, lg);
         dec_wait_lds();
         auto next = [&]() {
-            if (((blk + 1) & 31) == 0 && blk + 1 < nblk) load_ids(blk + 1);
-            issue(blk + 1);
+            if (((n + 1) & 31) == 0 && n + 1 < o.n) load_ids(n + 1);
+            issue(n + 1);
         };
         if constexpr (NT == 1) next();
 
-        const int at = p.p0 + 8 * blk + 2 * wave;
-        const bool two = at + 1 < p1;
+        const int at = p.p0 + 8 * o.block(n) + 2 * wave;
+        const bool two = !edge || at + 1 < p1;
         const int tok0 = sq.page(at) * kPage, tok1 = two ? sq.page(at + 1) * kPage : end;
         float x[NT][8];
 #pragma unroll
@@ -458,10 +479,8 @@ __device__ __forceinline__ void tree_piece(TreeShared<NT>& S, const TreePiece& p
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
-        // Which of the lane's 8 keys each of its rows sees (bits); all, in a block inside every row's keys.
-        auto inside = [&](int tk) { return tk + kPage <= full_hi && (tk >= full_lo || tk + kPage <= full_sink); };
-        const bool plain = two && inside(tok0) && inside(tok1);   // (uniform)
-        if (plain) {
+        // Which of the lane's 8 keys each of its rows sees (bits)
+        if constexpr (!edge) {
             if (biased) {
 #pragma unroll
                 for (int t = 0; t < NT; ++t)
@@ -584,7 +603,15 @@ __device__ __forceinline__ void tree_piece(TreeShared<NT>& S, const TreePiece& p
         for (int dt = 0; dt < 8; ++dt)
 #pragma unroll
             for (int t = 0; t < NT; ++t) acc[t][dt] = mfma16x16x32(b.v[dt], w[t], acc[t][dt]);
+    };
+
+    __syncthreads();   // mask rows and depths
+    if (o.n > 0) {
+        load_ids(0);
+        issue(0);
     }
+    for (int n = 0; n < o.plain; ++n) block(n, std::false_type{});
+    for (int n = o.plain; n < o.n; ++n) block(n, std::true_type{});
 
     // Join of the four waves: each leaves its output in its slot (row r's four dims c at place c ^ r of the row, so
     // that the 16 rows of a store lie in different banks).
@@ -606,7 +633,7 @@ __device__ __forceinline__ void tree_piece(TreeShared<NT>& S, const TreePiece& p
     const auto& f = *tree_args();
     const int kvh_ = (int)tree_fresh_s(blockIdx.x) % f.Hkv;
     if (S.wild) {   // (uniform)
-        tree_piece_rows<NT, MOD>(S, p, kvh_, end);
+        tree_piece_rows<MOD>(S, p, kvh_, end);
         return;
     }
 #pragma unroll 1
@@ -644,9 +671,353 @@ __device__ __forceinline__ void tree_piece(TreeShared<NT>& S, const TreePiece& p
     }
 }
 
+// ---- many rows: the row-split body -----------------------------------------------------------------
+//
+// With 32 rows on each key the key-split body is bound by the bytes that its waves wait for (8 x 8192 tokens, 64
+// drafted at G = 4: 203 us, 338 TFLOP/s): every row group streams all K and V again. Here a workgroup holds 64 NT rows,
+// 16 NT in each wave, and all four waves read the same 64-key blocks, staged by direct loads into one of two LDS
+// buffers while the other is computed: one barrier a block, and no join at the end.
 template <int NT, bool MOD>
-__global__ __launch_bounds__(kTreeThreads, 2) void tree_split_kernel(TreeArgs a) {
-    __shared__ TreeShared<NT> S;
+__device__ __forceinline__ void tree_piece_wide(TreeWideShared<NT>& S, const TreePiece& p, int kvh) {
+    constexpr int ROWS = 64 * NT;
+    const auto& a = *tree_args();
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    const int l16 = lane & 15, lg = lane >> 4, G = a.G;
+    const TreeSeq& sq = p.q;
+    const int ctx = sq.ctx;
+
+    __syncthreads();   // the piece before is done with the LDS
+    if (tid == 0) S.wild = 0;
+    if (a.mask) {
+        for (int i = tid; i < p.tokens * kTreeMaskWords; i += kTreeThreads) {
+            const int r = i / kTreeMaskWords, w = i % kTreeMaskWords;
+            S.mask[r][w] = w < a.mask_words ? a.mask[(size_t)(p.q0 + p.i0 + r) * a.mask_words + w] : 0u;
+        }
+    }
+    if (MOD && a.depth)
+        for (int j = tid; j < min(sq.n, kTreeMaxTokens); j += kTreeThreads) S.depth[j] = tree_depth(a.depth[p.q0 + j]);
+
+    // Tile t of wave w is tile 4 t + w of the group's rows (so that few rows fill the first tiles of all waves).
+    pf16x8 q[NT][4];
+    int pos[NT];
+    float slope[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const int r = min(16 * (4 * t + wave) + l16, p.rows - 1);
+        const int i = r / G, h = kvh * G + (r - i * G);
+        const size_t row = (size_t)(p.q0 + p.i0 + i) * a.Hq + h;
+        const _Float16* qp = a.q + row * kHeadDim + 8 * lg;
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) q[t][ks] = *reinterpret_cast<const pf16x8*>(qp + 32 * ks);
+        pos[t] = MOD && a.depth ? tree_depth(a.depth[p.q0 + p.i0 + i]) : p.i0 + i;
+        slope[t] = MOD && a.slopes ? a.slopes[h] * kTreeLog2e : 0.f;
+        if (!MOD) dec_sign_q(q[t], a.scale_log2);
+    }
+    const TreeKeys ks = tree_keys<MOD>(a, p, lane);
+    const int end = ks.end, p1 = ks.p1;
+    const TreeOrder o = tree_order(p.p0, 4, 4, p1, ks.a0, ks.a1);
+
+    // Staging: wave w moves page w of every block, K and V; rows and swizzles as in tree_piece.
+    const uint32_t page_bytes = (uint32_t)(kPage * a.Hkv * 256);
+    const uint32_t kbase = (uint32_t)(lg * a.Hkv * 256 + ((l16 ^ lg) << 4)), vbase = (uint32_t)(lg * a.Hkv * 256 + ((l16 ^ (lg << 1)) << 4));
+    const uint32_t rows4 = (uint32_t)(4 * a.Hkv * 256);
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)S.block[0] + kDecPageBytes * wave;
+    const uint8_t* const kc = a.k + kvh * 256;
+    const uint8_t* const vc = a.v + kvh * 256;
+    int pidv = 0;   // lane x: this wave's page of the x-th block of a window of 64
+    auto load_ids = [&](int n) {
+        const int at = p.p0 + 4 * o.block(min(n + lane, o.n - 1)) + wave;
+        pidv = tree_args()->kv_indices[p.pb + sq.page(min(at, p1 - 1))];
+    };
+    auto issue = [&](int n) {
+        if (n >= o.n || p.p0 + 4 * o.block(n) + wave >= p1) return;
+        const uint32_t kb = tree_fresh(kbase), vb = tree_fresh(vbase);
+        const size_t off = (size_t)(uint32_t)__builtin_amdgcn_readlane(pidv, n & 63) * page_bytes;
+        const uint32_t lds = lds0 + (n & 1) * (8 * kDecPageBytes);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) dec_dma(kc + off, (kb ^ (uint32_t)(i << 6)) + i * rows4, lds + 1024 * i);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) dec_dma(vc + off, (vb ^ (uint32_t)((i & 1) << 7)) + i * rows4, lds + 4 * kDecPageBytes + 1024 * i);
+    };
+
+    uint32_t wild = 0u;
+    float m[NT], l[NT];
+    pf32x4 acc[NT][8];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        m[t] = -INFINITY;
+        l[t] = 0.f;
+#pragma unroll
+        for (int dt = 0; dt < 8; ++dt) acc[t][dt] = pf32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    const float scale2 = MOD ? 1.f : a.scale_log2 == 0.f ? 0x1p-126f : fabsf(a.scale_log2);
+
+    auto block = [&](int n, auto EDGE) {
+        constexpr bool edge = decltype(EDGE)::value;
+        typedef __attribute__((address_space(3))) uint8_t lds_u8;
+        if (((n + 1) & 63) == 0 && n + 1 < o.n) load_ids(n + 1);
+        issue(n + 1);
+        lds_u8* const buf = (lds_u8*)S.block[0] + (n & 1) * (8 * kDecPageBytes);
+        // S^T: x[t][4 tk + j] = score of key 16 tk + 4 lg + j and row l16 of tile t; K of tile tk + 1 is read before the
+        // MFMAs of tile tk
+        float x[NT][16];
+        const uint32_t kl = tree_fresh((uint32_t)(l16 * 256 + ((((l16 >> 2) << 2) | (lg ^ (l16 & 3))) << 4)));
+        auto kfrag = [&](int tk, pf16x8 (&ka)[4]) {
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks)
+                ka[ks] = __builtin_bit_cast(pf16x8, *(const __attribute__((address_space(3))) pu32x4*)(
+                                                        buf + ((kl ^ (uint32_t)(ks << 6)) + kDecPageBytes * tk)));
+        };
+        constexpr int AHEAD = edge ? 0 : 1;   // (an edge block's bits take the registers)
+        pf16x8 ka[1 + AHEAD][4];
+        if (AHEAD) kfrag(0, ka[0]);
+#pragma unroll
+        for (int tk = 0; tk < 4; ++tk) {
+            if (tk < 4 - AHEAD) kfrag(tk + AHEAD, ka[(tk + AHEAD) & AHEAD]);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                pf32x4 c = pf32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int ks = 0; ks < 4; ++ks) c = mfma16x16x32(ka[tk & AHEAD][ks], q[t][ks], c);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[t][4 * tk + j] = c[j];
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        const int at = p.p0 + 4 * o.block(n);
+        auto first_key = [&](int tk) { return sq.page(at + tk) * kPage; };
+        bool biased = false;
+        if constexpr (MOD) {
+            const auto& h = *tree_args();
+            const float cap_in = h.cap_in, cap_out = h.cap_out, scale_log2 = h.scale_log2;
+            biased = h.slopes != nullptr;
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                if (cap_out > 0.f) {   // (uniform)
+                    float top = 0.f;
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        x[t][e] *= cap_in;
+                        top = fmaxf(top, fabsf(x[t][e]));
+                    }
+                    if (__builtin_amdgcn_ballot_w64(!(top <= 1.f))) {
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            const float s = tree_tanh_small(x[t][e]), g = tree_tanh_large(x[t][e]);
+                            x[t][e] = cap_out * (fabsf(x[t][e]) <= 1.f ? s : g);
+                            __builtin_amdgcn_sched_barrier(0);
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) x[t][e] = cap_out * tree_tanh_small(x[t][e]);
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) x[t][e] *= scale_log2;
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        uint32_t keep[2][4];   // (edge) the V elements of real keys, per 32 keys
+        if constexpr (edge) {
+            const auto& f = *tree_args();
+            const int gs = __builtin_ctz(f.G), lg4 = (int)(tree_fresh(lane) >> 4) * 4;
+            auto below = [](int n) { return (1u << min(max(n, 0), 4)) - 1u; };
+            uint32_t real = 0u;
+            int k0[4];
+#pragma unroll
+            for (int tk = 0; tk < 4; ++tk) {
+                k0[tk] = (at + tk < p1 ? first_key(tk) : end) + lg4;
+                real |= below(end - k0[tk]) << (4 * tk);
+            }
+            uint32_t near[NT];
+#pragma unroll
+            for (int t = 0; t < NT; ++t) near[t] = 0xFFFFu;
+            if constexpr (MOD) {
+                const int window = f.window;
+                if (window > 0) {
+                    uint32_t kept = 0u;
+#pragma unroll
+                    for (int tk = 0; tk < 4; ++tk) kept |= below(f.sink - k0[tk]) << (4 * tk);
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) near[t] = kept;
+                }
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int at_key = tree_key_pos(f.depth != nullptr, S, k0[e >> 2] + (e & 3) - ctx);
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) {
+                        const int apart = pos[t] - at_key;
+                        near[t] |= (uint32_t)(apart - window) >> 31 << e;
+                        if (biased) x[t][e] = fmaf(slope[t], (float)-apart, x[t][e]);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                const int tok = min(16 * (4 * t + wave) + (int)(tree_fresh(lane) & 15u), p.rows - 1) >> gs;
+                uint32_t seen = 0u;
+                if (f.mask) {
+#pragma unroll
+                    for (int tk = 0; tk < 4; ++tk) {
+                        const int j = k0[tk] - ctx, w = j >> 5;
+                        const uint32_t* row = S.mask[tok];
+                        const uint32_t lo = w < 0 ? ~0u : row[min(w, kTreeMaskWords - 1)];
+                        const uint32_t hi = w < -1 ? ~0u : w + 1 < kTreeMaskWords ? row[w + 1] : 0u;
+                        seen |= (__builtin_amdgcn_alignbit(hi, lo, (uint32_t)j & 31u) & 15u) << (4 * tk);
+                    }
+                } else {
+#pragma unroll
+                    for (int tk = 0; tk < 4; ++tk) seen |= below(ctx + p.i0 + tok + 1 - k0[tk]) << (4 * tk);
+                }
+                seen &= real & near[t];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) x[t][e] = seen >> e & 1u ? x[t][e] : -INFINITY;
+                __builtin_amdgcn_sched_barrier(0);
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    keep[h][i] = ((uint32_t)((int)(real << (31 - 8 * h - 2 * i)) >> 31) & 0xFFFFu) |
+                                 ((uint32_t)((int)(real << (30 - 8 * h - 2 * i)) >> 31) & 0xFFFF0000u);
+        } else if (biased) {
+#pragma unroll
+            for (int tk = 0; tk < 4; ++tk) {
+                const int k0 = first_key(tk) + 4 * lg - ctx;
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) x[t][4 * tk + j] = fmaf(slope[t], (float)(k0 + j - pos[t]), x[t][4 * tk + j]);
+            }
+        }
+
+        // Online softmax in base 2, as in tree_piece.
+        float mn[NT];
+        bool grow = false;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            float mx = x[t][0];
+#pragma unroll
+            for (int e = 1; e < 16; ++e) mx = fmaxf(mx, x[t][e]);
+            mn[t] = fmaxf(m[t], col4_reduce<true>(mx));
+            grow |= mn[t] > m[t];
+        }
+        if (__builtin_amdgcn_ballot_w64(grow)) {
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                const float al = mn[t] > m[t] ? __builtin_amdgcn_exp2f((m[t] - mn[t]) * scale2) : 1.f;
+                l[t] *= al;
+#pragma unroll
+                for (int dt = 0; dt < 8; ++dt) acc[t][dt] *= al;
+                m[t] = mn[t];
+            }
+        }
+        pf16x8 w[NT][2];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const float ms = m[t] == -INFINITY ? 0.f : m[t];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const float pe = __builtin_amdgcn_exp2f(fmaf(x[t][e] - ms, scale2, 15.f));
+                l[t] += pe;
+                w[t][e >> 3][e & 7] = (_Float16)pe;
+            }
+        }
+
+        // O^T += V^T P^T, the fragments of dim tile dt + 1 read before the MFMAs of dt
+        const int vk = 4 * lg + (l16 >> 2);
+        const uint32_t vl = tree_fresh((uint32_t)(4 * kDecPageBytes + vk * 256 + ((((vk & 7) << 1) | ((l16 & 3) >> 1)) << 4) + 8 * (l16 & 1)));
+        auto vfrag = [&](int dt, int h) {
+            pf16x4 half[2];
+#pragma unroll
+            for (int y = 0; y < 2; ++y)
+                half[y] = __builtin_bit_cast(pf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16(
+                    (__attribute__((address_space(3))) lds_f16x4*)(buf + ((vl ^ (uint32_t)(dt << 5)) + kDecPageBytes * (2 * h + y)))));
+            return pf16x8{half[0][0], half[0][1], half[0][2], half[0][3], half[1][0], half[1][1], half[1][2], half[1][3]};
+        };
+        pf16x8 va[1 + AHEAD][2];
+        if (AHEAD) {
+            va[0][0] = vfrag(0, 0);
+            va[0][1] = vfrag(0, 1);
+        }
+#pragma unroll
+        for (int dt = 0; dt < 8; ++dt) {
+            if (dt < 8 - AHEAD) {
+                va[(dt + AHEAD) & AHEAD][0] = vfrag(dt + AHEAD, 0);
+                va[(dt + AHEAD) & AHEAD][1] = vfrag(dt + AHEAD, 1);
+            }
+            if constexpr (edge) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    pu32x4 u = __builtin_bit_cast(pu32x4, va[dt & AHEAD][h]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        u[i] &= keep[h][i];
+                        wild |= ((u[i] & 0x7C00u) == 0x7C00u) | ((u[i] & 0x7C000000u) == 0x7C000000u);
+                    }
+                    va[dt & AHEAD][h] = __builtin_bit_cast(pf16x8, u);
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int t = 0; t < NT; ++t) acc[t][dt] = mfma16x16x32(va[dt & AHEAD][h], w[t][h], acc[t][dt]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        dec_wait_loads();   // this wave's part of the next block
+        dec_barrier();
+    };
+
+    if (o.n > 0) {
+        load_ids(0);
+        issue(0);
+    }
+    dec_wait_loads();
+    __syncthreads();   // mask rows, depths, the first block
+    for (int n = 0; n < o.plain; ++n) block(n, std::false_type{});
+    for (int n = o.plain; n < o.n; ++n) block(n, std::true_type{});
+
+    if (__builtin_amdgcn_ballot_w64(wild != 0u) && lane == 0) S.wild = 1;
+    __syncthreads();
+    const auto& f = *tree_args();
+    const int kvh_ = (int)tree_fresh_s(blockIdx.x) % f.Hkv;
+    if (S.wild) {   // (uniform)
+        tree_piece_rows<MOD>(S, p, kvh_, end);
+        return;
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const float L = col4_reduce<false>(l[t]);
+        const int r = 16 * (4 * t + wave) + (int)(tree_fresh(lane) & 15u);
+        if (r >= p.rows) continue;
+        const float inv = L == 0.f ? 0.f : 1.f / L;
+        const float lse = L == 0.f ? -INFINITY : fmaf(m[t] == -INFINITY ? 0.f : m[t], scale2, __builtin_amdgcn_logf(L) - 15.f) * kTreeLn2;
+        if (p.slot < 0) {
+            const int i = r / f.G;
+            const size_t row = (size_t)(p.q0 + p.i0 + i) * f.Hq + kvh_ * f.G + (r - i * f.G);
+#pragma unroll
+            for (int dt = 0; dt < 8; ++dt) {
+                const pf32x4 o = acc[t][dt] * inv;
+                *reinterpret_cast<pf16x4*>(f.out + row * kHeadDim + 16 * dt + 4 * lg) =
+                    pf16x4{(_Float16)o[0], (_Float16)o[1], (_Float16)o[2], (_Float16)o[3]};
+            }
+            if (lg == 0) f.lse[row] = lse;
+        } else {
+            const size_t row = (size_t)p.slot * ROWS + r;
+#pragma unroll
+            for (int dt = 0; dt < 8; ++dt) *reinterpret_cast<pf32x4*>(f.part_o + row * kHeadDim + 16 * dt + 4 * lg) = acc[t][dt] * inv;
+            if (lg == 0) f.part_lse[row] = lse;
+        }
+    }
+}
+
+// A workgroup's range, piece by piece.
+template <class Sh, class Piece>
+__device__ __forceinline__ void tree_workgroup(const TreeArgs& a, Sh& S, Piece piece) {
     const int g = blockIdx.x / a.Hkv, kvh = blockIdx.x - g * a.Hkv;
     int64_t lo, hi, units;
     int ranges;
@@ -694,8 +1065,25 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_split_kernel(TreeArgs a)
         left -= take;
         skip = 0;
         ++j;
-        tree_piece<NT, MOD>(S, p, kvh);
+        // (kept in vector registers meanwhile, of which there are more)
+        const uint32_t left_ = tree_fresh((uint32_t)left), b_ = tree_fresh((uint32_t)b), j_ = tree_fresh((uint32_t)j);
+        piece(p, kvh);
+        left = (int)__builtin_amdgcn_readfirstlane(left_);
+        b = (int)__builtin_amdgcn_readfirstlane(b_);
+        j = (int)__builtin_amdgcn_readfirstlane(j_);
     }
+}
+
+template <int NT, bool MOD>
+__global__ __launch_bounds__(kTreeThreads, 2) void tree_split_kernel(TreeArgs a) {
+    __shared__ TreeSplitShared<NT> S;
+    tree_workgroup(a, S, [&](const TreePiece& p, int kvh) { tree_piece<NT, MOD>(S, p, kvh); });
+}
+template <int NT, bool MOD>
+__global__ __launch_bounds__(kTreeThreads, 2) void tree_wide_kernel(TreeArgs a) {
+    __shared__ TreeWideShared<NT> S;
+    static_assert(2 * sizeof(S) <= 160 * 1024, "two workgroups on a CU");
+    tree_workgroup(a, S, [&](const TreePiece& p, int kvh) { tree_piece_wide<NT, MOD>(S, p, kvh); });
 }
 
 // Merge of the cut items: boundary g, kv head, four rows a workgroup, a row per wave. Each half of a wave takes every
@@ -760,6 +1148,12 @@ void launch_tree_split(const TreeArgs& a, bool mod, hipStream_t s) {
     if (mod) tree_split_kernel<NT, true><<<W, kTreeThreads, 0, s>>>(a);
     else tree_split_kernel<NT, false><<<W, kTreeThreads, 0, s>>>(a);
 }
+template <int NT>
+void launch_tree_wide(const TreeArgs& a, bool mod, hipStream_t s) {
+    const int W = a.ranges * a.Hkv;
+    if (mod) tree_wide_kernel<NT, true><<<W, kTreeThreads, 0, s>>>(a);
+    else tree_wide_kernel<NT, false><<<W, kTreeThreads, 0, s>>>(a);
+}
 
 }  // namespace
 
@@ -768,6 +1162,8 @@ hipError_t launch_tree_attention(const TreeArgs& a, hipStream_t s) {
     const bool mod = a.cap_out > 0.f || a.slopes || a.window > 0;
     if (a.rows == 16) launch_tree_split<1>(a, mod, s);
     else if (a.rows == 32) launch_tree_split<2>(a, mod, s);
+    else if (a.rows == 64) launch_tree_wide<1>(a, mod, s);
+    else if (a.rows == 128) launch_tree_wide<2>(a, mod, s);
     else return hipErrorInvalidValue;
     if (a.ranges > 1) {
         const int most = std::min(a.rows, std::max(1, a.max_tokens) * a.G);

@@ -97,6 +97,8 @@ def test_attended_pages_hold_every_key_in_a_window(arith, seed):
     for pos in range(n):   # any position a token may have: ctx + a depth of 0 or more
         seen = [k for k in range(length) if window == 0 or k >= t["ctx"] + pos - window + 1 or k < sink]
         assert {k // 16 for k in seen} <= set(pages)
+    for page in range(np_ + 1):
+        assert arith.t_below(*args, page) == sum(x < page for x in pages)
     if window and t["ctx"] > window + sink + 64:
         assert len(pages) < np_
 
@@ -112,3 +114,21 @@ def test_attended_pages_hold_every_key_in_a_window(arith, seed):
 def test_tables_that_make_no_sense(arith, args, expect):
     t = _seq(arith, *args)
     assert {k: t[k] for k in expect} == expect
+
+
+@pytest.mark.parametrize("step,width", [(8, 2), (4, 4)])
+def test_order_of_blocks(arith, step, width):
+    """Every block once, the plain ones first and all of them, whatever the pages that every row sees."""
+    rng = np.random.default_rng(step)
+    out, order = (ctypes.c_int * 2)(), (ctypes.c_int * 200)()
+    plain_seen = 0
+    for _ in range(4000):
+        first, p1 = int(rng.integers(0, 40)), int(rng.integers(0, 120))
+        a0, a1 = sorted(rng.integers(-5, 140, 2).tolist()) if rng.random() < 0.8 else rng.integers(-5, 140, 2).tolist()
+        arith.t_order(first, step, width, p1, a0, a1, out, order)
+        n, plain = out
+        assert n == len(range(first, p1, step)) and sorted(order[:n]) == list(range(n)) and 0 <= plain <= n
+        want = [i for i in range(n) if a0 <= first + step * i and first + step * i + width <= min(a1, p1)]
+        assert sorted(order[:plain]) == want
+        plain_seen += plain
+    assert plain_seen > 1000
