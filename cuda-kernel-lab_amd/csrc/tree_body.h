@@ -56,15 +56,21 @@ struct TreeScan {
     int64_t wave[kTreeWaves];
     int64_t prefix;   // units before the range's first sequence
     int first;        // that sequence
+    int tables[5];    // and its entries, as TreeTables
 };
 
+// The entries of two sequences in the device's tables in one register, lanes 0 .. 4 and 8 .. 12: the first page-table
+// entries of the sequence and of the next, the tokens in its last page, the first tokens (rows of q) of it and of the next.
+// This lane's entry (lane & 7) of sequence b:
 template <class A>
-__device__ __forceinline__ TreeSeq tree_load_seq(const A& a, int b, int* q0, int* pb) {
-    const int ip0 = a.kv_indptr[b], ip1 = a.kv_indptr[b + 1], last = a.kv_last[b];
-    const int s0 = a.q_indptr ? a.q_indptr[b] : b, s1 = a.q_indptr ? a.q_indptr[b + 1] : b + 1;
-    *q0 = max(s0, 0);
-    *pb = ip0;
-    return tree_seq(ip0, ip1, last, s0, s1, a.n_tokens, a.tpg, a.window, a.sink);
+__device__ __forceinline__ int tree_load_entry(const A& a, int b, int lane) {
+    const int e = lane & 7;
+    b = min(b, a.B - 1);
+    const int32_t *last = a.kv_last, *ip = a.kv_indptr, *q = a.q_indptr;
+    const int32_t* p = e == 2 ? last + b : ip + b + (e == 1);
+    if (q && e > 2) p = q + b + (e == 4);
+    const int v = *p;
+    return e > 2 && !q ? b + (e == 4) : v;
 }
 
 __device__ __forceinline__ int64_t tree_shfl_up(int64_t v, int d) {
@@ -72,17 +78,35 @@ __device__ __forceinline__ int64_t tree_shfl_up(int64_t v, int d) {
     return (int64_t)(((uint64_t)(uint32_t)hi << 32) | (uint32_t)lo);
 }
 
-// Units of sequences 4 t .. 4 t + 3 of a pass (t = thread), the units before them in the pass, and the pass's sum.
-__device__ __forceinline__ int64_t tree_scan_pass(const TreeArgs& a, TreeScan& S, int b0, int64_t (&u)[kTreeScan], int64_t& sum) {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+__device__ __forceinline__ int64_t tree_uniform(int64_t v) {
+    return (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((int)v));
+}
+
+struct TreeFour {   // sequences 4 t .. 4 t + 3 of a pass, t the thread
+    int ip[kTreeScan + 1], last[kTreeScan], q[kTreeScan + 1];
+    int64_t u[kTreeScan];
+};
+
+// The units of the pass's sequences, those before the thread's, and the pass's sum. (All loads at clamped places, so that
+// none waits for another.)
+__device__ __forceinline__ int64_t tree_scan_pass(const TreeArgs& a, TreeScan& S, int b0, TreeFour& f, int64_t& sum) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, b = b0 + kTreeScan * tid;
+#pragma unroll
+    for (int k = 0; k <= kTreeScan; ++k) f.ip[k] = a.kv_indptr[min(b + k, a.B)];
+#pragma unroll
+    for (int k = 0; k <= kTreeScan; ++k) f.q[k] = min(b + k, a.B);
+    if (a.q_indptr) {
+#pragma unroll
+        for (int k = 0; k <= kTreeScan; ++k) f.q[k] = a.q_indptr[min(b + k, a.B)];
+    }
+#pragma unroll
+    for (int k = 0; k < kTreeScan; ++k) f.last[k] = a.kv_last[min(b + k, a.B - 1)];
     int64_t mine = 0;
 #pragma unroll
     for (int k = 0; k < kTreeScan; ++k) {
-        const int b = b0 + kTreeScan * tid + k;
-        int q0, pb;
-        const TreeSeq t = tree_load_seq(a, min(b, a.B - 1), &q0, &pb);
-        u[k] = b < a.B ? t.total() : 0;
-        mine += u[k];
+        const TreeSeq t = tree_seq(f.ip[k], f.ip[k + 1], f.last[k], f.q[k], f.q[k + 1], a.n_tokens, a.tpg, a.window, a.sink);
+        f.u[k] = b + k < a.B ? t.total() : 0;
+        mine += f.u[k];
     }
     int64_t x = mine;
 #pragma unroll
@@ -99,34 +123,41 @@ __device__ __forceinline__ int64_t tree_scan_pass(const TreeArgs& a, TreeScan& S
         before += w < wave ? S.wave[w] : 0;
         sum += S.wave[w];
     }
-    __syncthreads();
+    if (a.B > kTreeScan * kTreeThreads) __syncthreads();   // (S.wave is written again)
     return before + x - mine;
 }
 
 // The units [lo, hi) of range g, and where they start (in S). False: there is no such range.
 __device__ __forceinline__ bool tree_find_range(const TreeArgs& a, TreeScan& S, int g, int64_t& lo, int64_t& hi, int64_t& units, int& ranges) {
     constexpr int kPass = kTreeScan * kTreeThreads;
-    int64_t u[kTreeScan], sum, at = tree_scan_pass(a, S, 0, u, sum);
+    TreeFour f;
+    int64_t sum, at = tree_scan_pass(a, S, 0, f, sum);
     units = sum;
     for (int b0 = kPass; b0 < a.B; b0 += kPass) {
-        (void)tree_scan_pass(a, S, b0, u, sum);
+        (void)tree_scan_pass(a, S, b0, f, sum);
         units += sum;
     }
+    units = tree_uniform(units);
     ranges = units > 0 ? tree_ranges(units, a.ranges, a.least_units) : 0;
     if (g >= ranges) return false;
     lo = tree_range_start(units, ranges, g);
     hi = tree_range_start(units, ranges, g + 1);
     int64_t before = 0;
     for (int b0 = 0; b0 < a.B; b0 += kPass) {
-        if (a.B > kPass) at = tree_scan_pass(a, S, b0, u, sum);
+        if (a.B > kPass) at = tree_scan_pass(a, S, b0, f, sum);
         int64_t p = before + at;
 #pragma unroll
         for (int k = 0; k < kTreeScan; ++k) {
-            if (p <= lo && lo < p + u[k]) {
+            if (p <= lo && lo < p + f.u[k]) {
                 S.prefix = p;
                 S.first = b0 + kTreeScan * (int)threadIdx.x + k;
+                S.tables[0] = f.ip[k];
+                S.tables[1] = f.ip[k + 1];
+                S.tables[2] = f.last[k];
+                S.tables[3] = f.q[k];
+                S.tables[4] = f.q[k + 1];
             }
-            p += u[k];
+            p += f.u[k];
         }
         before += sum;
     }
@@ -143,7 +174,7 @@ struct TreeCommon {
     uint32_t mask[ROWS][kTreeMaskWords];                    // the group's mask rows
     int depth[kTreeMaxTokens];                              // the sequence's drafted tokens' depths
     TreeScan scan;
-    int wild;                                               // the piece goes row by row (tree_piece_rows)
+    int wild[2];                                            // the piece goes row by row (tree_piece_rows)
 };
 // The key-split body: 16 NT rows, every wave all of them.
 template <int NT>
@@ -204,6 +235,19 @@ struct TreePiece {
     int i0, tokens, rows;  // the group's first token within the sequence, its tokens and rows
     int p0, p1;            // attended pages of the piece
     int slot;              // partial slot, or -1
+    int par;               // which of the flags (TreeCommon) is the piece's
+};
+
+// What of a piece is needed again only at its end, or in few blocks, read from the lanes where tree_workgroup keeps it.
+struct TreeCold {
+    int v;
+    __device__ __forceinline__ int i0() const { return __builtin_amdgcn_readlane(v, 20); }
+    __device__ __forceinline__ int rows() const { return __builtin_amdgcn_readlane(v, 21); }
+    __device__ __forceinline__ int q0() const { return __builtin_amdgcn_readlane(v, 22); }
+    __device__ __forceinline__ int slot() const { return __builtin_amdgcn_readlane(v, 23); }
+    __device__ __forceinline__ int tokens() const { return __builtin_amdgcn_readlane(v, 24); }
+    // of the piece (20 .. 24 as above; 19: the next piece's flag)
+    __device__ __forceinline__ int flag() const { return ~__builtin_amdgcn_readlane(v, 19) & 1; }
 };
 
 // (so that sums of positions fit an int)
@@ -247,29 +291,69 @@ __device__ __forceinline__ TreeKeys tree_keys(const A& a, const TreePiece& p, in
     return k;
 }
 
+// The mask rows of the group and the depths of the sequence's drafted tokens into LDS, for pieces that hold drafted keys:
+// loaded by the first of these, stored by the second, with other loads started in between.
+template <int ROWS>
+struct TreeStage {
+    uint32_t m[ROWS * kTreeMaskWords / kTreeThreads];
+    int d[kTreeMaxTokens / kTreeThreads];
+};
+template <bool MOD, int ROWS, class A>
+__device__ __forceinline__ void tree_stage_load(TreeStage<ROWS>& g, const A& a, const TreePiece& p) {
+    const int tid = (int)tree_fresh(threadIdx.x);
+    if (a.mask) {
+#pragma unroll
+        for (int k = 0; k < ROWS * kTreeMaskWords / kTreeThreads; ++k) {
+            const int r = min((tid + k * kTreeThreads) / kTreeMaskWords, p.tokens - 1), w = tid % kTreeMaskWords;
+            const uint32_t v = a.mask[(size_t)(p.q0 + p.i0 + r) * a.mask_words + min(w, a.mask_words - 1)];
+            g.m[k] = w < a.mask_words ? v : 0u;
+        }
+    }
+    if (MOD && a.depth) {
+#pragma unroll
+        for (int k = 0; k < kTreeMaxTokens / kTreeThreads; ++k) {
+            g.d[k] = a.depth[p.q0 + min(tid + k * kTreeThreads, p.q.n - 1)];
+        }
+    }
+}
+template <bool MOD, class Sh, class A>
+__device__ __forceinline__ void tree_stage_store(Sh& S, const TreeStage<Sh::ROWS>& g, const A& a) {
+    const int tid = (int)tree_fresh(threadIdx.x);
+    if (a.mask) {
+#pragma unroll
+        for (int k = 0; k < Sh::ROWS * kTreeMaskWords / kTreeThreads; ++k)
+            S.mask[(tid + k * kTreeThreads) / kTreeMaskWords][tid % kTreeMaskWords] = g.m[k];
+    }
+    if (MOD && a.depth) {
+#pragma unroll
+        for (int k = 0; k < kTreeMaxTokens / kTreeThreads; ++k) S.depth[tid + k * kTreeThreads] = tree_depth(g.d[k]);
+    }
+}
+
 // A piece row by row, for one thing alone: V of a key that some rows see and others do not holds NaN or infinity, which
 // a product with the weight 0 of those others would pass on. A wave per row, 64 keys at a time: a key per lane for
 // the scores, then two dims per lane, over the keys that the row sees.
 template <bool MOD, class Sh>
-__device__ __forceinline__ void tree_piece_rows(Sh& S, const TreePiece& p, int kvh, int end) {
+__device__ __forceinline__ void tree_piece_rows(Sh& S, const TreePiece& p, int kvh, int end, TreeCold cold) {
     constexpr int ROWS = Sh::ROWS;
     const auto& a = *tree_args();
     const int wave = __builtin_amdgcn_readfirstlane(tree_fresh(threadIdx.x) >> 6), lane = (int)(tree_fresh(threadIdx.x) & 63u);
     const TreeSeq& sq = p.q;
+    const int rows = cold.rows(), i0 = cold.i0(), q0 = cold.q0(), slot = cold.slot();
     float* const sp = reinterpret_cast<float*>(S.scratch(wave));          // the weights of 64 keys, then their pages
     int* const spg = reinterpret_cast<int*>(S.scratch(wave)) + 64;
     __syncthreads();   // the waves' outputs in the slots are given up
-    for (int r = wave; r < p.rows; r += kTreeWaves) {
+    for (int r = wave; r < rows; r += kTreeWaves) {
         const int i = r / a.G, h = kvh * a.G + (r - i * a.G);
-        const size_t row = (size_t)(p.q0 + p.i0 + i) * a.Hq + h;
+        const size_t row = (size_t)(q0 + i0 + i) * a.Hq + h;
         const _Float16* q = a.q + row * kHeadDim;
-        const int pos = MOD && a.depth ? tree_depth(a.depth[p.q0 + p.i0 + i]) : p.i0 + i;
+        const int pos = MOD && a.depth ? tree_depth(a.depth[q0 + i0 + i]) : i0 + i;
         const float slope = MOD && a.slopes ? a.slopes[h] * kTreeLog2e : 0.f;
         float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
         for (int at = p.p0; at < p.p1; at += 4) {   // four pages
             const int mine = at + (lane >> 4), page = sq.page(min(mine, p.p1 - 1)), key = page * kPage + (lane & 15), j = key - sq.ctx;
             bool seen = mine < p.p1 && key < end;
-            if (seen && j >= 0) seen = a.mask ? (S.mask[i][min(j, kTreeMaxTokens - 1) >> 5] >> (j & 31) & 1u) != 0u : j <= p.i0 + i;
+            if (seen && j >= 0) seen = a.mask ? (S.mask[i][min(j, kTreeMaxTokens - 1) >> 5] >> (j & 31) & 1u) != 0u : j <= i0 + i;
             const int apart = pos - (MOD ? tree_key_pos(a.depth != nullptr, S, j) : j);
             if (MOD && a.window > 0) seen = seen && (apart < a.window || key < a.sink);
             const int id = a.kv_indices[p.pb + page];
@@ -316,12 +400,12 @@ __device__ __forceinline__ void tree_piece_rows(Sh& S, const TreePiece& p, int k
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) l += __shfl_xor(l, d, 64);
         const float inv = l == 0.f ? 0.f : 1.f / l, lse = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kTreeLn2;
-        if (p.slot < 0) {
+        if (slot < 0) {
             a.out[row * kHeadDim + 2 * lane] = (_Float16)(o0 * inv);
             a.out[row * kHeadDim + 2 * lane + 1] = (_Float16)(o1 * inv);
             if (lane == 0) a.lse[row] = lse;
         } else {
-            const size_t pr = (size_t)p.slot * ROWS + r;
+            const size_t pr = (size_t)slot * ROWS + r;
             *reinterpret_cast<float2*>(a.part_o + pr * kHeadDim + 2 * lane) = make_float2(o0 * inv, o1 * inv);
             if (lane == 0) a.part_lse[pr] = lse;
         }
@@ -329,7 +413,7 @@ __device__ __forceinline__ void tree_piece_rows(Sh& S, const TreePiece& p, int k
 }
 
 template <int NT, bool MOD>
-__device__ __forceinline__ void tree_piece(TreeSplitShared<NT>& S, const TreePiece& p, int kvh) {
+__device__ __forceinline__ void tree_piece(TreeSplitShared<NT>& S, const TreePiece& p, int kvh, TreeCold cold) {
     constexpr int ROWS = 16 * NT;
     const auto& a = *tree_args();
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
@@ -338,32 +422,9 @@ __device__ __forceinline__ void tree_piece(TreeSplitShared<NT>& S, const TreePie
     const int ctx = sq.ctx;
 
     __syncthreads();   // the piece before is done with the LDS
-    if (tid == 0) S.wild = 0;
-    if (a.mask) {
-        for (int i = tid; i < p.tokens * kTreeMaskWords; i += kTreeThreads) {
-            const int r = i / kTreeMaskWords, w = i % kTreeMaskWords;
-            S.mask[r][w] = w < a.mask_words ? a.mask[(size_t)(p.q0 + p.i0 + r) * a.mask_words + w] : 0u;
-        }
-    }
-    if (MOD && a.depth)
-        for (int j = tid; j < min(sq.n, kTreeMaxTokens); j += kTreeThreads) S.depth[j] = tree_depth(a.depth[p.q0 + j]);
+    if (tid == 0) S.wild[p.par ^ 1] = 0;   // the next piece's
+    PD_STAMP(2 + 8 * p.par);
 
-    // This lane's row of each tile: token i0 + r / G, head kvh G + r % G (rows past the group repeat its last)
-    pf16x8 q[NT][4];
-    int pos[NT];   // the token's position relative to the context
-    float slope[NT];
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        const int r = min(16 * t + l16, p.rows - 1);
-        const int i = r / G, h = kvh * G + (r - i * G);
-        const size_t row = (size_t)(p.q0 + p.i0 + i) * a.Hq + h;
-        const _Float16* qp = a.q + row * kHeadDim + 8 * lg;
-#pragma unroll
-        for (int ks = 0; ks < 4; ++ks) q[t][ks] = *reinterpret_cast<const pf16x8*>(qp + 32 * ks);
-        pos[t] = MOD && a.depth ? tree_depth(a.depth[p.q0 + p.i0 + i]) : p.i0 + i;
-        slope[t] = MOD && a.slopes ? a.slopes[h] * kTreeLog2e : 0.f;
-        if (!MOD) dec_sign_q(q[t], a.scale_log2);
-    }
     const TreeKeys ks = tree_keys<MOD>(a, p, lane);
     const int end = ks.end, p1 = ks.p1;
     const TreeOrder o = tree_order(p.p0 + 2 * wave, 8, 2, p1, ks.a0, ks.a1);
@@ -397,6 +458,30 @@ __device__ __forceinline__ void tree_piece(TreeSplitShared<NT>& S, const TreePie
         }
     };
 
+    // The page ids, then the q and mask rows on the way, then the first block's loads as soon as the ids are there
+    if (o.n > 0) load_ids(0);
+    // This lane's row of each tile: token i0 + r / G, head kvh G + r % G (rows past the group repeat its last)
+    pf16x8 q[NT][4];
+    int pos[NT];   // the token's position relative to the context
+    float slope[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const int r = min(16 * t + l16, p.rows - 1);
+        const int i = r / G, h = kvh * G + (r - i * G);
+        const size_t row = (size_t)(p.q0 + p.i0 + i) * a.Hq + h;
+        const _Float16* qp = a.q + row * kHeadDim + 8 * lg;
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) q[t][ks] = *reinterpret_cast<const pf16x8*>(qp + 32 * ks);
+        pos[t] = MOD && a.depth ? tree_depth(a.depth[p.q0 + p.i0 + i]) : p.i0 + i;
+        slope[t] = MOD && a.slopes ? a.slopes[h] * kTreeLog2e : 0.f;
+        if (!MOD) dec_sign_q(q[t], a.scale_log2);
+    }
+    const bool drafts = p1 > p.p0 && (sq.page(p1 - 1) + 1) * kPage > ctx;   // (uniform) the piece holds drafted keys
+    TreeStage<ROWS> stage;
+    if (drafts) tree_stage_load<MOD>(stage, a, p);
+    if (o.n > 0) issue(0);
+    PD_STAMP(3 + 8 * p.par);
+    if (drafts) tree_stage_store<MOD>(S, stage, a);
     uint32_t wild = 0u;   // not 0: an element of V, of a key that not every row may see, is not finite
     float m[NT], l[NT];
     pf32x4 acc[NT][8];
@@ -523,7 +608,7 @@ __device__ __forceinline__ void tree_piece(TreeSplitShared<NT>& S, const TreePie
             if (f.mask) {
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
-                    const int tok = min(16 * t + (int)(tree_fresh(lane) & 15u), p.rows - 1) >> gs;
+                    const int tok = min(16 * t + (int)(tree_fresh(lane) & 15u), cold.rows() - 1) >> gs;
                     // 4 bits from drafted token j on; those before the first are cached keys, seen
                     auto bits = [&](int j) {
                         const int w = j >> 5;
@@ -538,7 +623,7 @@ __device__ __forceinline__ void tree_piece(TreeSplitShared<NT>& S, const TreePie
             } else {
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
-                    const int upto = ctx + p.i0 + (min(16 * t + (int)(tree_fresh(lane) & 15u), p.rows - 1) >> gs) + 1;
+                    const int upto = ctx + cold.i0() + (min(16 * t + (int)(tree_fresh(lane) & 15u), cold.rows() - 1) >> gs) + 1;
                     seen[t] = real & near[t] & (below(upto - k0) | below(upto - k1) << 4);
                 }
             }
@@ -605,18 +690,16 @@ __device__ __forceinline__ void tree_piece(TreeSplitShared<NT>& S, const TreePie
             for (int t = 0; t < NT; ++t) acc[t][dt] = mfma16x16x32(b.v[dt], w[t], acc[t][dt]);
     };
 
-    __syncthreads();   // mask rows and depths
-    if (o.n > 0) {
-        load_ids(0);
-        issue(0);
-    }
+    if (drafts) __syncthreads();   // mask rows and depths
+    PD_STAMP(4 + 8 * cold.flag());
     for (int n = 0; n < o.plain; ++n) block(n, std::false_type{});
     for (int n = o.plain; n < o.n; ++n) block(n, std::true_type{});
+    PD_STAMP(5 + 8 * cold.flag());
 
     // Join of the four waves: each leaves its output in its slot (row r's four dims c at place c ^ r of the row, so
     // that the 16 rows of a store lie in different banks).
     dec_wait_lds();
-    if (__builtin_amdgcn_ballot_w64(wild != 0u) && lane == 0) S.wild = 1;
+    if (__builtin_amdgcn_ballot_w64(wild != 0u) && lane == 0) S.wild[cold.flag()] = 1;
     float* const so = reinterpret_cast<float*>(S.slot[wave]);
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
@@ -632,14 +715,15 @@ __device__ __forceinline__ void tree_piece(TreeSplitShared<NT>& S, const TreePie
     __syncthreads();
     const auto& f = *tree_args();
     const int kvh_ = (int)tree_fresh_s(blockIdx.x) % f.Hkv;
-    if (S.wild) {   // (uniform)
-        tree_piece_rows<MOD>(S, p, kvh_, end);
+    if (S.wild[cold.flag()]) {   // (uniform)
+        tree_piece_rows<MOD>(S, p, kvh_, end, cold);
         return;
     }
+    const int rows = cold.rows(), slot = cold.slot(), token0 = cold.q0() + cold.i0();
 #pragma unroll 1
     for (int it = 0; it < ROWS * 32 / kTreeThreads; ++it) {
         const int idx = it * kTreeThreads + (int)tree_fresh(threadIdx.x), r = idx >> 5, c = idx & 31;
-        if (r >= p.rows) continue;
+        if (r >= rows) continue;
         float mw[kTreeWaves], M = -INFINITY, L = 0.f;
         pf32x4 o = pf32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -657,14 +741,14 @@ __device__ __forceinline__ void tree_piece(TreeSplitShared<NT>& S, const TreePie
         }
         const float inv = L == 0.f ? 0.f : 1.f / L;
         const float lse = L == 0.f ? -INFINITY : fmaf(M, scale2, __builtin_amdgcn_logf(L) - 15.f) * kTreeLn2;
-        if (p.slot < 0) {
+        if (slot < 0) {
             const int i = r / f.G;
-            const size_t row = (size_t)(p.q0 + p.i0 + i) * f.Hq + kvh_ * f.G + (r - i * f.G);
+            const size_t row = (size_t)(token0 + i) * f.Hq + kvh_ * f.G + (r - i * f.G);
             const pf16x4 h = {(_Float16)(o[0] * inv), (_Float16)(o[1] * inv), (_Float16)(o[2] * inv), (_Float16)(o[3] * inv)};
             *reinterpret_cast<pf16x4*>(f.out + row * kHeadDim + 4 * c) = h;
             if (c == 0) f.lse[row] = lse;
         } else {
-            const size_t row = (size_t)p.slot * ROWS + r;
+            const size_t row = (size_t)slot * ROWS + r;
             *reinterpret_cast<pf32x4*>(f.part_o + row * kHeadDim + 4 * c) = o * inv;
             if (c == 0) f.part_lse[row] = lse;
         }
@@ -678,7 +762,7 @@ __device__ __forceinline__ void tree_piece(TreeSplitShared<NT>& S, const TreePie
 // 16 NT in each wave, and all four waves read the same 64-key blocks, staged by direct loads into one of two LDS
 // buffers while the other is computed: one barrier a block, and no join at the end.
 template <int NT, bool MOD>
-__device__ __forceinline__ void tree_piece_wide(TreeWideShared<NT>& S, const TreePiece& p, int kvh) {
+__device__ __forceinline__ void tree_piece_wide(TreeWideShared<NT>& S, const TreePiece& p, int kvh, TreeCold cold) {
     constexpr int ROWS = 64 * NT;
     const auto& a = *tree_args();
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
@@ -687,32 +771,9 @@ __device__ __forceinline__ void tree_piece_wide(TreeWideShared<NT>& S, const Tre
     const int ctx = sq.ctx;
 
     __syncthreads();   // the piece before is done with the LDS
-    if (tid == 0) S.wild = 0;
-    if (a.mask) {
-        for (int i = tid; i < p.tokens * kTreeMaskWords; i += kTreeThreads) {
-            const int r = i / kTreeMaskWords, w = i % kTreeMaskWords;
-            S.mask[r][w] = w < a.mask_words ? a.mask[(size_t)(p.q0 + p.i0 + r) * a.mask_words + w] : 0u;
-        }
-    }
-    if (MOD && a.depth)
-        for (int j = tid; j < min(sq.n, kTreeMaxTokens); j += kTreeThreads) S.depth[j] = tree_depth(a.depth[p.q0 + j]);
+    if (tid == 0) S.wild[p.par ^ 1] = 0;   // the next piece's
+    PD_STAMP(2 + 8 * p.par);
 
-    // Tile t of wave w is tile 4 t + w of the group's rows (so that few rows fill the first tiles of all waves).
-    pf16x8 q[NT][4];
-    int pos[NT];
-    float slope[NT];
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        const int r = min(16 * (4 * t + wave) + l16, p.rows - 1);
-        const int i = r / G, h = kvh * G + (r - i * G);
-        const size_t row = (size_t)(p.q0 + p.i0 + i) * a.Hq + h;
-        const _Float16* qp = a.q + row * kHeadDim + 8 * lg;
-#pragma unroll
-        for (int ks = 0; ks < 4; ++ks) q[t][ks] = *reinterpret_cast<const pf16x8*>(qp + 32 * ks);
-        pos[t] = MOD && a.depth ? tree_depth(a.depth[p.q0 + p.i0 + i]) : p.i0 + i;
-        slope[t] = MOD && a.slopes ? a.slopes[h] * kTreeLog2e : 0.f;
-        if (!MOD) dec_sign_q(q[t], a.scale_log2);
-    }
     const TreeKeys ks = tree_keys<MOD>(a, p, lane);
     const int end = ks.end, p1 = ks.p1;
     const TreeOrder o = tree_order(p.p0, 4, 4, p1, ks.a0, ks.a1);
@@ -740,6 +801,29 @@ __device__ __forceinline__ void tree_piece_wide(TreeWideShared<NT>& S, const Tre
         for (int i = 0; i < 4; ++i) dec_dma(vc + off, (vb ^ (uint32_t)((i & 1) << 7)) + i * rows4, lds + 4 * kDecPageBytes + 1024 * i);
     };
 
+    if (o.n > 0) load_ids(0);
+    // Tile t of wave w is tile 4 t + w of the group's rows (so that few rows fill the first tiles of all waves).
+    pf16x8 q[NT][4];
+    int pos[NT];
+    float slope[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const int r = min(16 * (4 * t + wave) + l16, p.rows - 1);
+        const int i = r / G, h = kvh * G + (r - i * G);
+        const size_t row = (size_t)(p.q0 + p.i0 + i) * a.Hq + h;
+        const _Float16* qp = a.q + row * kHeadDim + 8 * lg;
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) q[t][ks] = *reinterpret_cast<const pf16x8*>(qp + 32 * ks);
+        pos[t] = MOD && a.depth ? tree_depth(a.depth[p.q0 + p.i0 + i]) : p.i0 + i;
+        slope[t] = MOD && a.slopes ? a.slopes[h] * kTreeLog2e : 0.f;
+        if (!MOD) dec_sign_q(q[t], a.scale_log2);
+    }
+    const bool drafts = p1 > p.p0 && (sq.page(p1 - 1) + 1) * kPage > ctx;   // (uniform) the piece holds drafted keys
+    TreeStage<ROWS> stage;
+    if (drafts) tree_stage_load<MOD>(stage, a, p);
+    if (o.n > 0) issue(0);
+    PD_STAMP(3 + 8 * p.par);
+    if (drafts) tree_stage_store<MOD>(S, stage, a);
     uint32_t wild = 0u;
     float m[NT], l[NT];
     pf32x4 acc[NT][8];
@@ -857,7 +941,7 @@ __device__ __forceinline__ void tree_piece_wide(TreeWideShared<NT>& S, const Tre
             }
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
-                const int tok = min(16 * (4 * t + wave) + (int)(tree_fresh(lane) & 15u), p.rows - 1) >> gs;
+                const int tok = min(16 * (4 * t + wave) + (int)(tree_fresh(lane) & 15u), cold.rows() - 1) >> gs;
                 uint32_t seen = 0u;
                 if (f.mask) {
 #pragma unroll
@@ -870,7 +954,7 @@ __device__ __forceinline__ void tree_piece_wide(TreeWideShared<NT>& S, const Tre
                     }
                 } else {
 #pragma unroll
-                    for (int tk = 0; tk < 4; ++tk) seen |= below(ctx + p.i0 + tok + 1 - k0[tk]) << (4 * tk);
+                    for (int tk = 0; tk < 4; ++tk) seen |= below(ctx + cold.i0() + tok + 1 - k0[tk]) << (4 * tk);
                 }
                 seen &= real & near[t];
 #pragma unroll
@@ -972,33 +1056,32 @@ __device__ __forceinline__ void tree_piece_wide(TreeWideShared<NT>& S, const Tre
         dec_barrier();
     };
 
-    if (o.n > 0) {
-        load_ids(0);
-        issue(0);
-    }
     dec_wait_loads();
     __syncthreads();   // mask rows, depths, the first block
+    PD_STAMP(4 + 8 * cold.flag());
     for (int n = 0; n < o.plain; ++n) block(n, std::false_type{});
     for (int n = o.plain; n < o.n; ++n) block(n, std::true_type{});
+    PD_STAMP(5 + 8 * cold.flag());
 
-    if (__builtin_amdgcn_ballot_w64(wild != 0u) && lane == 0) S.wild = 1;
+    if (__builtin_amdgcn_ballot_w64(wild != 0u) && lane == 0) S.wild[cold.flag()] = 1;
     __syncthreads();
     const auto& f = *tree_args();
     const int kvh_ = (int)tree_fresh_s(blockIdx.x) % f.Hkv;
-    if (S.wild) {   // (uniform)
-        tree_piece_rows<MOD>(S, p, kvh_, end);
+    if (S.wild[cold.flag()]) {   // (uniform)
+        tree_piece_rows<MOD>(S, p, kvh_, end, cold);
         return;
     }
+    const int rows = cold.rows(), slot = cold.slot(), token0 = cold.q0() + cold.i0();
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
         const float L = col4_reduce<false>(l[t]);
         const int r = 16 * (4 * t + wave) + (int)(tree_fresh(lane) & 15u);
-        if (r >= p.rows) continue;
+        if (r >= rows) continue;
         const float inv = L == 0.f ? 0.f : 1.f / L;
         const float lse = L == 0.f ? -INFINITY : fmaf(m[t] == -INFINITY ? 0.f : m[t], scale2, __builtin_amdgcn_logf(L) - 15.f) * kTreeLn2;
-        if (p.slot < 0) {
+        if (slot < 0) {
             const int i = r / f.G;
-            const size_t row = (size_t)(p.q0 + p.i0 + i) * f.Hq + kvh_ * f.G + (r - i * f.G);
+            const size_t row = (size_t)(token0 + i) * f.Hq + kvh_ * f.G + (r - i * f.G);
 #pragma unroll
             for (int dt = 0; dt < 8; ++dt) {
                 const pf32x4 o = acc[t][dt] * inv;
@@ -1007,7 +1090,7 @@ __device__ __forceinline__ void tree_piece_wide(TreeWideShared<NT>& S, const Tre
             }
             if (lg == 0) f.lse[row] = lse;
         } else {
-            const size_t row = (size_t)p.slot * ROWS + r;
+            const size_t row = (size_t)slot * ROWS + r;
 #pragma unroll
             for (int dt = 0; dt < 8; ++dt) *reinterpret_cast<pf32x4*>(f.part_o + row * kHeadDim + 16 * dt + 4 * lg) = acc[t][dt] * inv;
             if (lg == 0) f.part_lse[row] = lse;
@@ -1018,7 +1101,12 @@ __device__ __forceinline__ void tree_piece_wide(TreeWideShared<NT>& S, const Tre
 // A workgroup's range, piece by piece.
 template <class Sh, class Piece>
 __device__ __forceinline__ void tree_workgroup(const TreeArgs& a, Sh& S, Piece piece) {
+    // timestamps (timeline build only), the last two pieces': 0 start, 1 the range found; with par the piece's flag, 2 + 8
+    // par begun, 3 + 8 par the first loads issued, 4 + 8 par at the first block, 5 + 8 par the blocks done, 6 + 8 par
+    // written; 31 end
+    PD_STAMP(0);
     const int g = blockIdx.x / a.Hkv, kvh = blockIdx.x - g * a.Hkv;
+    if (threadIdx.x == 0) S.wild[0] = 0;
     int64_t lo, hi, units;
     int ranges;
     const bool some = tree_find_range(a, S.scan, g, lo, hi, units, ranges);
@@ -1027,31 +1115,45 @@ __device__ __forceinline__ void tree_workgroup(const TreeArgs& a, Sh& S, Piece p
         return;
     }
     // The first item, the units of it before the range, and (kv head 0) what the merge has to know: an item that
-    // the boundary before this range is the first to cut, and its pieces.
+    // the boundary before this range cuts, which of its cuts that is, and its pieces.
+    PD_STAMP(1);
+    const int lane = threadIdx.x & 63;
     int b = __builtin_amdgcn_readfirstlane(S.scan.first), j, skip;
-    int left = (int)(hi - lo);
+    int left = __builtin_amdgcn_readfirstlane((int)(hi - lo));
+    // (the half of the entries' register that holds sequence b's)
+    const int after = tree_load_entry(*tree_args(), b + 1, lane);
+    int half = 0, entries = S.scan.tables[min(lane, 4)];
+    entries = lane < 8 ? entries : after;
+    auto entry = [&](int i) { return __builtin_amdgcn_readlane(entries, half + i); };
+    auto sequence = [&](const auto& k) {
+        return tree_seq(entry(0), entry(1), entry(2), entry(3), entry(4), k.n_tokens, k.tpg, k.window, k.sink);
+    };
     {
         const auto& k = *tree_args();
-        int q0, pb;
-        const TreeSeq t = tree_load_seq(k, b, &q0, &pb);
-        const int64_t in = lo - S.scan.prefix;
-        j = (int)(in / t.units());
-        skip = (int)(in - (int64_t)j * t.units());
+        const TreeSeq t = sequence(k);
+        const int64_t in = lo - tree_uniform(S.scan.prefix);
+        j = __builtin_amdgcn_readfirstlane((int)(in / t.units()));
+        skip = __builtin_amdgcn_readfirstlane((int)(in - (int64_t)j * t.units()));
         if (kvh == 0 && threadIdx.x == 0) {
             const int64_t first = lo - skip;
             const int g0 = tree_range_of(units, ranges, first), g1 = tree_range_of(units, ranges, first + t.units() - 1);
             const int i0 = j * k.tpg;
-            k.cuts[g] = make_int4(q0 + i0, min(k.tpg, t.n - i0) * k.G, skip > 0 && g0 == g - 1 ? g1 - g0 + 1 : 0, 0);
+            k.cuts[g] = make_int4(max(entry(3), 0) + i0, min(k.tpg, t.n - i0) * k.G, skip > 0 ? g1 - g0 + 1 : 0, g - g0 - 1);
         }
     }
+    int par = 0;
     while (left > 0) {
         TreePiece p;
         const auto& k = *tree_args();
-        if (b >= k.B) break;   // (not reached: the units of the items from here on are at least `left`)
-        p.q = tree_load_seq(k, b, &p.q0, &p.pb);
+        p.q = sequence(k);
+        p.pb = entry(0);
+        p.q0 = max(entry(3), 0);
         if (j >= p.q.groups) {
-            ++b;
+            if (++b >= k.B) break;   // (not reached: the units of the items from here on are at least `left`)
             j = 0;
+            const int x = (int)tree_fresh((uint32_t)lane), v = tree_load_entry(k, b + 1, x);
+            entries = (x & 8) == half ? v : entries;
+            half ^= 8;
             continue;
         }
         const int take = min(left, p.q.units() - skip);
@@ -1062,41 +1164,51 @@ __device__ __forceinline__ void tree_workgroup(const TreeArgs& a, Sh& S, Piece p
         p.p1 = min(skip + take, p.q.attended());
         const int s = tree_slot(skip, take, p.q.units());
         p.slot = s < 0 ? -1 : 2 * (int)blockIdx.x + s;
+        p.par = par;
         left -= take;
         skip = 0;
         ++j;
-        // (kept in vector registers meanwhile, of which there are more)
-        const uint32_t left_ = tree_fresh((uint32_t)left), b_ = tree_fresh((uint32_t)b), j_ = tree_fresh((uint32_t)j);
-        piece(p, kvh);
-        left = (int)__builtin_amdgcn_readfirstlane(left_);
-        b = (int)__builtin_amdgcn_readfirstlane(b_);
-        j = (int)__builtin_amdgcn_readfirstlane(j_);
+        par ^= 1;
+        // (the loop's own state is kept in lanes of the entries' register meanwhile)
+        const uint32_t x = tree_fresh((uint32_t)lane);
+        entries = x < 16 ? entries : x == 16 ? left : x == 17 ? b : x == 18 ? j : x == 19 ? half | par
+                : x == 20 ? p.i0 : x == 21 ? p.rows : x == 22 ? p.q0 : x == 23 ? p.slot : p.tokens;
+        entries = (int)tree_fresh((uint32_t)entries);
+        piece(p, kvh, entries);
+        left = __builtin_amdgcn_readlane(entries, 16);
+        b = __builtin_amdgcn_readlane(entries, 17);
+        j = __builtin_amdgcn_readlane(entries, 18);
+        half = __builtin_amdgcn_readlane(entries, 19) & 8;
+        par = __builtin_amdgcn_readlane(entries, 19) & 1;
+        PD_STAMP(6 + 8 * (par ^ 1));
     }
+    PD_STAMP(31);
 }
 
 template <int NT, bool MOD>
 __global__ __launch_bounds__(kTreeThreads, 2) void tree_split_kernel(TreeArgs a) {
     __shared__ TreeSplitShared<NT> S;
-    tree_workgroup(a, S, [&](const TreePiece& p, int kvh) { tree_piece<NT, MOD>(S, p, kvh); });
+    tree_workgroup(a, S, [&](const TreePiece& p, int kvh, int cold) { tree_piece<NT, MOD>(S, p, kvh, {cold}); });
 }
 template <int NT, bool MOD>
 __global__ __launch_bounds__(kTreeThreads, 2) void tree_wide_kernel(TreeArgs a) {
     __shared__ TreeWideShared<NT> S;
     static_assert(2 * sizeof(S) <= 160 * 1024, "two workgroups on a CU");
-    tree_workgroup(a, S, [&](const TreePiece& p, int kvh) { tree_piece_wide<NT, MOD>(S, p, kvh); });
+    tree_workgroup(a, S, [&](const TreePiece& p, int kvh, int cold) { tree_piece_wide<NT, MOD>(S, p, kvh, {cold}); });
 }
 
-// Merge of the cut items: boundary g, kv head, four rows a workgroup, a row per wave. Each half of a wave takes every
-// second piece, four dims a lane, in order; the halves are joined at the end (a fixed order).
+// Merge of the cut items. Boundary g, kv head: of the item that it cuts (pieces n: cut cut.w of n - 1) every (n - 1)-th
+// row, a row per wave. Each half of a wave takes every second piece, four dims a lane, in order; the halves are joined
+// at the end (a fixed order).
 __global__ __launch_bounds__(kTreeThreads) void tree_merge_kernel(TreeArgs a, int ROWS) {
     const int g = blockIdx.x / a.Hkv + 1, kvh = blockIdx.x % a.Hkv;
     const int4 cut = a.cuts[g];
-    const int n = cut.z;
+    const int n = cut.z, g0 = g - 1 - cut.w;
     if (n == 0) return;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, half = lane >> 5, c = lane & 31;
-    for (int r = blockIdx.y * kTreeWaves + wave; r < cut.y; r += gridDim.y * kTreeWaves) {
-        // piece k: range g - 1 + k, slot 1 of the first's workgroup, slot 0 of the others'
-        auto slot = [&](int k) { return ((size_t)((g - 1 + k) * a.Hkv + kvh) * 2 + (k == 0)) * ROWS + r; };
+    for (int r = cut.w + (n - 1) * (int)(blockIdx.y * kTreeWaves + wave); r < cut.y; r += (n - 1) * (int)gridDim.y * kTreeWaves) {
+        // piece k: range g0 + k, slot 1 of the first's workgroup, slot 0 of the others'
+        auto slot = [&](int k) { return ((size_t)((g0 + k) * a.Hkv + kvh) * 2 + (k == 0)) * ROWS + r; };
         float m = -INFINITY, ws = 0.f;
         pf32x4 o = pf32x4{0.f, 0.f, 0.f, 0.f};
         constexpr int U = 4;
@@ -1167,7 +1279,8 @@ hipError_t launch_tree_attention(const TreeArgs& a, hipStream_t s) {
     else return hipErrorInvalidValue;
     if (a.ranges > 1) {
         const int most = std::min(a.rows, std::max(1, a.max_tokens) * a.G);
-        tree_merge_kernel<<<dim3((a.ranges - 1) * a.Hkv, (most + kTreeWaves - 1) / kTreeWaves), kTreeThreads, 0, s>>>(a, a.rows);
+        // (four rows a wave at most: a row is a round trip or two)
+        tree_merge_kernel<<<dim3((a.ranges - 1) * a.Hkv, (most + 4 * kTreeWaves - 1) / (4 * kTreeWaves)), kTreeThreads, 0, s>>>(a, a.rows);
     }
     return hipGetLastError();
 }
