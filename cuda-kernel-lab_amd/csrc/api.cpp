@@ -1706,9 +1706,11 @@ int pdattn_tree_attention(const pdattn_tree_params* p, void* out, float* lse, pd
     a.max_tokens = p->q_indptr ? p->max_tokens : 1;
     a.mask_words = p->mask_words;
     a.rows = L.rows;
-    a.tpg = L.rows / G;
+    a.tl = __builtin_ctz((unsigned)(L.rows / G));   // (both powers of two)
     a.ranges = L.ranges;
     a.least_units = 8;
+    a.early = L.rows <= 32 ? 9 : 1;
+    a.late = L.rows <= 32 ? 8 : 1;
     a.window = std::min(p->score.window, 1 << 30);   // (past any position: sums of positions fit an int)
     a.sink = std::min(p->score.sink, 1 << 30);
     a.scale_log2 = p->sm_scale * 1.4426950408889634f;

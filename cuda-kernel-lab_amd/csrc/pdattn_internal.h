@@ -212,8 +212,9 @@ struct TreeArgs {
     float*          part_o;       // [2 ranges Hkv, rows, 128] partial outputs (normalized), tree_arith.h's slots
     float*          part_lse;     // [2 ranges Hkv, rows]
     int B, Hq, Hkv, G, n_tokens, max_tokens, mask_words, window, sink;
-    int rows, tpg;                // rows of a workgroup, tokens of a group (rows / G)
+    int rows, tl;                 // rows of a workgroup; 2^tl tokens of a group: rows / G
     int ranges, least_units;      // ranges of the grid, and units that a range has at least
+    int early, late;              // lengths of the first half of the ranges to the others'
     float scale_log2;             // sm_scale log2(e)
     float cap_in, cap_out;        // sm_scale / cap and cap log2(e), or 0
 };

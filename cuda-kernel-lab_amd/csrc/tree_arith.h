@@ -3,10 +3,10 @@
 //
 // The rows of a sequence for one kv head (its n tokens times the G query heads of the head, a token's heads
 // together) are cut into groups of as many tokens as fill a workgroup's rows. Each (sequence, group) is an item; its
-// units are the pages that the sequence attends. The units of all items, in the order of sequences, groups and
-// pages, are cut into equal ranges, and workgroup (g, kv head) takes range g: pieces of items, one after the
-// other. An item inside one range is written by its workgroup. Of an item cut by range boundaries, the piece that
-// starts it goes to partial slot 2 w + 1 of its workgroup w = g Hkv + kv head, every later piece to slot 2 w of its.
+// units are the pages that its tokens may see. The units of all items, in the order of sequences, groups and pages, are
+// cut into ranges, and workgroup (g, kv head) takes range g: pieces of items, one after the other. An item inside one
+// range is written by its workgroup. Of an item cut by range boundaries, the piece that starts it goes to partial
+// slot 2 w + 1 of its workgroup w = g Hkv + kv head, every later piece to slot 2 w of its.
 #pragma once
 
 #include <cstdint>
@@ -15,30 +15,56 @@
 
 namespace pdattn {
 
+// x / d for x >= 0, d > 0: in 32 bits where they hold x (a 64-bit division is some hundred instructions).
+PD_RANGE_FN int64_t tree_div(int64_t x, int64_t d) {
+    return (uint64_t)x >> 32 || (uint64_t)d >> 32 ? x / d : (int64_t)((uint32_t)x / (uint32_t)d);
+}
+
 // One sequence of the batch as the kernels see it. Positions count from the sequence's first cached token.
 struct TreeSeq {
     int len, n, ctx;     // cached tokens, new ones among them, those before them (below 0: n > len)
     int np;              // pages
     int s, w0;           // attended pages: [0, s) and [w0, np)
     int groups;
-    // attended pages, and the units of one of its items: a sequence without pages still has its rows to write
+    // units of group j: u0 + st (j >> cl). Chains: later tokens see more pages, a page more every 16 tokens.
+    int u0, st, cl;
     PD_RANGE_FN int attended() const { return s + np - w0; }
-    PD_RANGE_FN int units() const { return attended() > 0 ? attended() : 1; }
-    PD_RANGE_FN int64_t total() const { return (int64_t)groups * units(); }
     // the page at place i of the attended ones
     PD_RANGE_FN int page(int i) const { return i < s ? i : i - s + w0; }
+    // the places of pages below page p (those before it in the order of places)
+    PD_RANGE_FN int below(int p) const { return p <= s ? p : p <= w0 ? s : s + p - w0; }
+    PD_RANGE_FN int units(int j) const { return u0 + st * (j >> cl); }
+    // units of the groups before j
+    PD_RANGE_FN int64_t before(int j) const {
+        if (st == 0) return (int64_t)u0 * j;
+        const int64_t m = j >> cl;
+        return (int64_t)u0 * j + st * ((m * (m - 1) / 2 << cl) + (j - (m << cl)) * m);
+    }
+    PD_RANGE_FN int64_t total() const { return before(groups); }
+    // the group that holds the sequence's unit x
+    PD_RANGE_FN int group_of(int64_t x) const {
+        if (groups <= 1) return 0;
+        if (st == 0) return (int)tree_div(x, u0);
+        int lo = 0, hi = groups - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) / 2;
+            if (before(mid) <= x) lo = mid;
+            else hi = mid - 1;
+        }
+        return lo;
+    }
 };
 
-// From the device's tables as they are (no trust in them: never a negative count). page_tokens = 16; tpg: tokens
-// per group.
-PD_RANGE_FN TreeSeq tree_seq(int ip0, int ip1, int last, int q0, int q1, int n_tokens, int tpg, int window, int sink) {
+// From the device's tables as they are (no trust in them: never a negative count). 2^tl tokens per group; causal: no
+// token sees drafted keys after its own.
+PD_RANGE_FN TreeSeq tree_seq(int ip0, int ip1, int last, int q0, int q1, int n_tokens, int tl, int window, int sink, bool causal) {
     TreeSeq t;
     t.np = ip1 > ip0 ? ip1 - ip0 : 0;
     t.len = t.np > 0 ? (t.np - 1) * 16 + (last < 1 ? 1 : last > 16 ? 16 : last) : 0;
     const int a = q0 < 0 ? 0 : q0 > n_tokens ? n_tokens : q0, b = q1 < 0 ? 0 : q1 > n_tokens ? n_tokens : q1;
     t.n = b > a ? b - a : 0;
     t.ctx = t.len - t.n;
-    t.groups = (t.n + tpg - 1) / tpg;
+    t.groups = (int)(((int64_t)t.n + (1 << tl) - 1) >> tl);
     t.s = t.w0 = 0;
     if (window > 0) {
         // a token at position ctx or later sees, below the context, only keys from ctx - window + 1 on
@@ -50,11 +76,21 @@ PD_RANGE_FN TreeSeq tree_seq(int ip0, int ip1, int last, int q0, int q1, int n_t
             t.w0 = w0;
         }
     }
+    // A sequence without pages still has its rows to write: one unit an item at least.
+    t.u0 = t.attended() > 0 ? t.attended() : 1;
+    t.st = 0;
+    t.cl = 0;
+    if (causal && t.groups > 1 && t.ctx >= 0 && (int64_t)2 * t.n > t.ctx) {
+        // Tokens of group j see the keys below ctx + (j + 1) 2^tl. (Where the context is most of them, equal units are
+        // better: the groups' cuts then fall on the same keys, which their workgroups read together, through one L2. A
+        // chain of 512 on 2 x 8192 tokens: 164 us, with their own units 191.)
+        const int sl = tl > 4 ? tl : 4;   // a step is 16 tokens or a group
+        t.u0 = t.below((t.ctx + (1 << sl) + 15) >> 4);
+        t.st = 1 << (sl - 4);
+        t.cl = sl - tl;
+    }
     return t;
 }
-
-// The attended pages of a sequence below page `p` (those before it in the order of places).
-PD_RANGE_FN int tree_places_below(const TreeSeq& t, int p) { return p <= t.s ? p : p <= t.w0 ? t.s : t.s + p - t.w0; }
 
 // The blocks of a wave: block i starts at place first + step i and has `width` places, those below p1. Places [a0, a1) hold
 // pages whose every key is seen by every row: the blocks inside them are `plain`, and come first; then those behind
@@ -74,16 +110,35 @@ PD_RANGE_FN TreeOrder tree_order(int first, int step, int width, int p1, int a0,
     return o;
 }
 
-// Ranges that `units` are cut into: at most `most`, of at least `least` units each.
-PD_RANGE_FN int tree_ranges(int64_t units, int most, int least) {
-    const int64_t r = units / least;
-    return r < 1 ? 1 : r > most ? most : (int)r;
+// The cut of `units` into ranges: at most `most`, of at least `least` units on average. With two workgroups on a CU the
+// one that came first issues first: where all `most` ranges are used, the first half of them is longer, `early` to
+// `late`.
+struct TreeCuts {
+    int64_t units;
+    int ranges, early, late, half, total;   // half: ranges of the first kind; total: the sum of their weights
+    PD_RANGE_FN int64_t start(int g) const {
+        const int w = g <= half ? early * g : early * half + late * (g - half);
+        return tree_div(units * w, total);
+    }
+    // the range that holds unit x
+    PD_RANGE_FN int of(int64_t x) const {
+        const int y = (int)tree_div((x + 1) * total - 1, units);
+        return y < early * half ? (int)((uint32_t)y / (uint32_t)early) : half + (int)((uint32_t)(y - early * half) / (uint32_t)late);
+    }
+};
+PD_RANGE_FN TreeCuts tree_cuts(int64_t units, int most, int least, int early, int late) {
+    TreeCuts c;
+    c.units = units;
+    const int64_t r = tree_div(units, least);
+    c.ranges = units <= 0 ? 0 : r < 1 ? 1 : r > most ? most : (int)r;
+    c.half = c.ranges == most ? most / 2 : 0;
+    c.early = early;
+    c.late = c.half > 0 ? late : 1;
+    c.total = c.half > 0 ? early * c.half + late * (c.ranges - c.half) : c.ranges;
+    return c;
 }
-PD_RANGE_FN int64_t tree_range_start(int64_t units, int ranges, int g) { return units * g / ranges; }
-// The range that holds unit x.
-PD_RANGE_FN int tree_range_of(int64_t units, int ranges, int64_t x) { return (int)(((x + 1) * ranges - 1) / units); }
 
-// The partial slot of a piece that starts `skip` units into its item and takes `take` of its `units`, or -1: the
+// The partial slot (0 or 1) of a piece that starts `skip` units into its item and takes `take` of its `units`, or -1: the
 // whole item.
 PD_RANGE_FN int tree_slot(int skip, int take, int units) { return skip > 0 ? 0 : take < units ? 1 : -1; }
 

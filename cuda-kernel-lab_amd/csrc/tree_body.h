@@ -56,8 +56,13 @@ struct TreeScan {
     int64_t wave[kTreeWaves];
     int64_t prefix;   // units before the range's first sequence
     int first;        // that sequence
-    int tables[5];    // and its entries, as TreeTables
+    int tables[5];    // and its entries, as tree_load_entry
 };
+
+template <class A>
+__device__ __forceinline__ TreeSeq tree_seq_of(const A& a, int ip0, int ip1, int last, int q0, int q1) {
+    return tree_seq(ip0, ip1, last, q0, q1, a.n_tokens, a.tl, a.window, a.sink, a.mask == nullptr);
+}
 
 // The entries of two sequences in the device's tables in one register, lanes 0 .. 4 and 8 .. 12: the first page-table
 // entries of the sequence and of the next, the tokens in its last page, the first tokens (rows of q) of it and of the next.
@@ -77,9 +82,12 @@ __device__ __forceinline__ int64_t tree_shfl_up(int64_t v, int d) {
     const int lo = __shfl_up((int)v, d, 64), hi = __shfl_up((int)(v >> 32), d, 64);
     return (int64_t)(((uint64_t)(uint32_t)hi << 32) | (uint32_t)lo);
 }
-
 __device__ __forceinline__ int64_t tree_uniform(int64_t v) {
     return (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((int)v));
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int tree_dpp_add(int v) {   // + the value that the DPP step brings, 0 where it brings none
+    return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false);
 }
 
 struct TreeFour {   // sequences 4 t .. 4 t + 3 of a pass, t the thread
@@ -104,8 +112,7 @@ __device__ __forceinline__ int64_t tree_scan_pass(const TreeArgs& a, TreeScan& S
     int64_t mine = 0;
 #pragma unroll
     for (int k = 0; k < kTreeScan; ++k) {
-        const TreeSeq t = tree_seq(f.ip[k], f.ip[k + 1], f.last[k], f.q[k], f.q[k + 1], a.n_tokens, a.tpg, a.window, a.sink);
-        f.u[k] = b + k < a.B ? t.total() : 0;
+        f.u[k] = b + k < a.B ? tree_seq_of(a, f.ip[k], f.ip[k + 1], f.last[k], f.q[k], f.q[k + 1]).total() : 0;
         mine += f.u[k];
     }
     int64_t x = mine;
@@ -123,32 +130,77 @@ __device__ __forceinline__ int64_t tree_scan_pass(const TreeArgs& a, TreeScan& S
         before += w < wave ? S.wave[w] : 0;
         sum += S.wave[w];
     }
-    if (a.B > kTreeScan * kTreeThreads) __syncthreads();   // (S.wave is written again)
+    __syncthreads();   // (S.wave may be written again)
     return before + x - mine;
 }
 
-// The units [lo, hi) of range g, and where they start (in S). False: there is no such range.
-__device__ __forceinline__ bool tree_find_range(const TreeArgs& a, TreeScan& S, int g, int64_t& lo, int64_t& hi, int64_t& units, int& ranges) {
+// Range g of the batch.
+struct TreeRange {
+    TreeCuts cuts;
+    int64_t lo;       // its first unit
+    int64_t in;       // that unit within sequence b
+    int b, left;      // and the units of the range
+    int entries;      // of sequences b and b + 1, as tree_load_entry
+};
+__device__ __forceinline__ bool tree_find_range(const TreeArgs& a, TreeScan& S, int g, TreeRange& r) {
+    const int lane = threadIdx.x & 63;
+    if (a.B <= 64) {
+        // A sequence per lane, in every wave by itself: no barrier, and 32 bits while no sequence has 2^24 units
+        const int b = min(lane, a.B - 1);
+        const int32_t *ip = a.kv_indptr, *q = a.q_indptr;
+        const int ip0 = ip[b], ip1 = ip[b + 1], last = a.kv_last[b];
+        int q0 = b, q1 = b + 1;
+        if (q) {
+            q0 = q[b];
+            q1 = q[b + 1];
+        }
+        const int64_t mine = lane < a.B ? tree_seq_of(a, ip0, ip1, last, q0, q1).total() : 0;
+        if (!__builtin_amdgcn_ballot_w64(mine >> 24 != 0)) {
+            int x = (int)mine;   // inclusive sums: within rows of 16 lanes, then from row to row
+            x = tree_dpp_add<0x111, 0xF>(x);
+            x = tree_dpp_add<0x112, 0xF>(x);
+            x = tree_dpp_add<0x114, 0xF>(x);
+            x = tree_dpp_add<0x118, 0xF>(x);
+            x = tree_dpp_add<0x142, 0xA>(x);
+            x = tree_dpp_add<0x143, 0xC>(x);
+            r.cuts = tree_cuts(__builtin_amdgcn_readlane(x, 63), a.ranges, a.least_units, a.early, a.late);
+            if (g >= r.cuts.ranges) return false;
+            r.lo = r.cuts.start(g);
+            r.left = (int)(r.cuts.start(g + 1) - r.lo);
+            const int before = x - (int)mine, lo = (int)r.lo;
+            const uint64_t here = __builtin_amdgcn_ballot_w64(before <= lo && lo < x);
+            r.b = here ? __builtin_ctzll(here) : 0;   // (one bit)
+            r.in = lo - __builtin_amdgcn_readlane(before, r.b);
+            const int n = min(r.b + 1, a.B - 1);
+            const int e = lane & 7;
+            auto of = [&](int i) {
+                const int u0 = __builtin_amdgcn_readlane(ip0, i), u1 = __builtin_amdgcn_readlane(ip1, i), u2 = __builtin_amdgcn_readlane(last, i);
+                const int u3 = __builtin_amdgcn_readlane(q0, i), u4 = __builtin_amdgcn_readlane(q1, i);
+                return e == 0 ? u0 : e == 1 ? u1 : e == 2 ? u2 : e == 3 ? u3 : u4;
+            };
+            const int e0 = of(r.b), e1 = of(n);
+            r.entries = lane & 8 ? e1 : e0;
+            return true;
+        }
+    }
     constexpr int kPass = kTreeScan * kTreeThreads;
     TreeFour f;
-    int64_t sum, at = tree_scan_pass(a, S, 0, f, sum);
-    units = sum;
+    int64_t sum, at = tree_scan_pass(a, S, 0, f, sum), units = sum;
     for (int b0 = kPass; b0 < a.B; b0 += kPass) {
         (void)tree_scan_pass(a, S, b0, f, sum);
         units += sum;
     }
-    units = tree_uniform(units);
-    ranges = units > 0 ? tree_ranges(units, a.ranges, a.least_units) : 0;
-    if (g >= ranges) return false;
-    lo = tree_range_start(units, ranges, g);
-    hi = tree_range_start(units, ranges, g + 1);
+    r.cuts = tree_cuts(tree_uniform(units), a.ranges, a.least_units, a.early, a.late);
+    if (g >= r.cuts.ranges) return false;
+    r.lo = r.cuts.start(g);
+    r.left = __builtin_amdgcn_readfirstlane((int)(r.cuts.start(g + 1) - r.lo));
     int64_t before = 0;
     for (int b0 = 0; b0 < a.B; b0 += kPass) {
         if (a.B > kPass) at = tree_scan_pass(a, S, b0, f, sum);
         int64_t p = before + at;
 #pragma unroll
         for (int k = 0; k < kTreeScan; ++k) {
-            if (p <= lo && lo < p + f.u[k]) {
+            if (p <= r.lo && r.lo < p + f.u[k]) {
                 S.prefix = p;
                 S.first = b0 + kTreeScan * (int)threadIdx.x + k;
                 S.tables[0] = f.ip[k];
@@ -162,6 +214,11 @@ __device__ __forceinline__ bool tree_find_range(const TreeArgs& a, TreeScan& S, 
         before += sum;
     }
     __syncthreads();
+    r.b = __builtin_amdgcn_readfirstlane(S.first);
+    r.in = r.lo - tree_uniform(S.prefix);
+    const int after = tree_load_entry(a, r.b + 1, lane);
+    r.entries = S.tables[min(lane & 7, 4)];
+    r.entries = lane & 8 ? after : r.entries;
     return true;
 }
 
@@ -201,6 +258,32 @@ __device__ __forceinline__ uint32_t tree_fresh(uint32_t v) {
 __device__ __forceinline__ uint32_t tree_fresh_s(uint32_t v) {
     asm volatile("" : "+s"(v));
     return v;
+}
+
+// The online softmax, in base 2. A row's reference m is a score that is at most kTreeLag (in the exponent) below the
+// largest yet: it, and with it the sum and the output, moves only when a block passes that. So most blocks need neither the
+// maximum over a row's four lanes nor a rescaling (with the exact maximum, 8 x 8192 tokens and 64 drafted: 113.5 us, the
+// rescaling taken by about half of the blocks). A weight is exp2(score - m + kTreeShift), at most 2^15: fp16 holds it in
+// full down to 2^-21 of the reference's weight and to within 2^-32 of it below; l, of the weights in 32 bits, carries the
+// same factor.
+constexpr float kTreeLag = 8.f, kTreeShift = 7.f;
+template <int N>
+__device__ __forceinline__ float tree_largest(const float (&x)[N]) {
+    float mx = x[0];
+#pragma unroll
+    for (int e = 1; e < N; ++e) mx = fmaxf(mx, x[e]);
+    return mx;
+}
+// The lag in scores (finite: -infinity plus it stays).
+__device__ __forceinline__ float tree_slack(float scale2) { return fminf(kTreeLag / scale2, 1e38f); }
+__device__ __forceinline__ float tree_offset(float m, float scale2) { return m == -INFINITY ? kTreeShift : fmaf(-m, scale2, kTreeShift); }
+__device__ __forceinline__ void tree_grow(float mx, float& m, float& l, pf32x4 (&acc)[8], float scale2) {
+    const float mn = fmaxf(m, col4_reduce<true>(mx));
+    const float al = mn > m ? __builtin_amdgcn_exp2f((m - mn) * scale2) : 1.f;
+    l *= al;
+#pragma unroll
+    for (int dt = 0; dt < 8; ++dt) acc[dt] *= al;
+    m = mn;
 }
 
 // A block's operands from the wave's slot, as dec_read_block (of which they are the halves).
@@ -245,10 +328,14 @@ struct TreeCold {
     __device__ __forceinline__ int rows() const { return __builtin_amdgcn_readlane(v, 21); }
     __device__ __forceinline__ int q0() const { return __builtin_amdgcn_readlane(v, 22); }
     __device__ __forceinline__ int slot() const { return __builtin_amdgcn_readlane(v, 23); }
-    __device__ __forceinline__ int tokens() const { return __builtin_amdgcn_readlane(v, 24); }
-    // of the piece (20 .. 24 as above; 19: the next piece's flag)
+    // the workgroup is of the second half of the grid
+    __device__ __forceinline__ int late() const { return __builtin_amdgcn_readlane(v, 24); }
+    // (lane 19: the next piece's flag)
     __device__ __forceinline__ int flag() const { return ~__builtin_amdgcn_readlane(v, 19) & 1; }
 };
+
+// Not 0 where one of two fp16 is infinite or NaN: exponents of ones carry into the sign's place.
+__device__ __forceinline__ uint32_t tree_not_finite(uint32_t w) { return ((w & 0x7C007C00u) + 0x04000400u) & 0x80008000u; }
 
 // (so that sums of positions fit an int)
 __device__ __forceinline__ int tree_depth(int d) { return min(max(d, 0), 1 << 28); }
@@ -271,7 +358,7 @@ __device__ __forceinline__ TreeKeys tree_keys(const A& a, const TreePiece& p, in
     const bool tree = a.mask || a.depth;
     k.end = a.mask ? sq.len : min(sq.len, sq.ctx + p.i0 + p.tokens);
     if (tree) k.end = min(k.end, sq.ctx + kTreeMaxTokens);
-    k.p1 = min(p.p1, tree_places_below(sq, max(0, (k.end + kPage - 1) / kPage)));
+    k.p1 = min(p.p1, sq.below(max(0, (k.end + kPage - 1) / kPage)));
     // of the keys below `hi` every row sees those from `lo` on: the window's start at the last position of the group
     const int hi = tree ? sq.ctx : sq.ctx + p.i0 + 1;
     int lo = 0;
@@ -286,8 +373,8 @@ __device__ __forceinline__ TreeKeys tree_keys(const A& a, const TreePiece& p, in
         }
         lo = max(0, sq.ctx + last - a.window + 1);
     }
-    k.a0 = tree_places_below(sq, (lo + kPage - 1) / kPage);
-    k.a1 = tree_places_below(sq, max(0, hi) / kPage);
+    k.a0 = sq.below((lo + kPage - 1) / kPage);
+    k.a1 = sq.below(max(0, hi) / kPage);
     return k;
 }
 
@@ -493,7 +580,7 @@ __device__ __forceinline__ void tree_piece(TreeSplitShared<NT>& S, const TreePie
         for (int dt = 0; dt < 8; ++dt) acc[t][dt] = pf32x4{0.f, 0.f, 0.f, 0.f};
     }
     // (a scale of 0 would make an unseen key's -inf a NaN)
-    const float scale2 = MOD ? 1.f : a.scale_log2 == 0.f ? 0x1p-126f : fabsf(a.scale_log2);
+    const float scale2 = MOD ? 1.f : a.scale_log2 == 0.f ? 0x1p-126f : fabsf(a.scale_log2), slack = tree_slack(scale2);
 
     auto block = [&](int n, auto EDGE) {
         constexpr bool edge = decltype(EDGE)::value;
@@ -644,42 +731,29 @@ __device__ __forceinline__ void tree_piece(TreeSplitShared<NT>& S, const TreePie
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     w[i] &= keep[i];
-                    odd |= ((w[i] & 0x7C00u) == 0x7C00u) | ((w[i] & 0x7C000000u) == 0x7C000000u);
+                    odd |= tree_not_finite(w[i]);
                 }
                 b.v[dt] = __builtin_bit_cast(pf16x8, w);
+                odd = tree_fresh(odd);
             }
             wild |= odd;
         }
 
-        // Online softmax in base 2. The weights carry a factor 2^15, in l and in the PV product alike, so that fp16
-        // holds them down to 2^-39 of the running maximum's.
-        float mn[NT];
+        // Online softmax (tree_grow)
         bool grow = false;
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            float mx = x[t][0];
-#pragma unroll
-            for (int e = 1; e < 8; ++e) mx = fmaxf(mx, x[t][e]);
-            mn[t] = fmaxf(m[t], col4_reduce<true>(mx));
-            grow |= mn[t] > m[t];
-        }
+        for (int t = 0; t < NT; ++t) grow |= tree_largest<8>(x[t]) > m[t] + slack;
         if (__builtin_amdgcn_ballot_w64(grow)) {
 #pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                const float al = mn[t] > m[t] ? __builtin_amdgcn_exp2f((m[t] - mn[t]) * scale2) : 1.f;
-                l[t] *= al;
-#pragma unroll
-                for (int dt = 0; dt < 8; ++dt) acc[t][dt] *= al;
-                m[t] = mn[t];
-            }
+            for (int t = 0; t < NT; ++t) tree_grow(tree_largest<8>(x[t]), m[t], l[t], acc[t], scale2);
         }
         pf16x8 w[NT];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-            const float ms = m[t] == -INFINITY ? 0.f : m[t];
+            const float c = tree_offset(m[t], scale2);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const float pe = __builtin_amdgcn_exp2f(fmaf(x[t][e] - ms, scale2, 15.f));
+                const float pe = __builtin_amdgcn_exp2f(fmaf(x[t][e], scale2, c));
                 l[t] += pe;
                 w[t][e] = (_Float16)pe;
             }
@@ -740,7 +814,7 @@ __device__ __forceinline__ void tree_piece(TreeSplitShared<NT>& S, const TreePie
             for (int j = 0; j < 4; ++j) o[j] = fmaf(al, v[j], o[j]);
         }
         const float inv = L == 0.f ? 0.f : 1.f / L;
-        const float lse = L == 0.f ? -INFINITY : fmaf(M, scale2, __builtin_amdgcn_logf(L) - 15.f) * kTreeLn2;
+        const float lse = L == 0.f ? -INFINITY : fmaf(M, scale2, __builtin_amdgcn_logf(L) - kTreeShift) * kTreeLn2;
         if (slot < 0) {
             const int i = r / f.G;
             const size_t row = (size_t)(token0 + i) * f.Hq + kvh_ * f.G + (r - i * f.G);
@@ -834,11 +908,18 @@ __device__ __forceinline__ void tree_piece_wide(TreeWideShared<NT>& S, const Tre
 #pragma unroll
         for (int dt = 0; dt < 8; ++dt) acc[t][dt] = pf32x4{0.f, 0.f, 0.f, 0.f};
     }
-    const float scale2 = MOD ? 1.f : a.scale_log2 == 0.f ? 0x1p-126f : fabsf(a.scale_log2);
+    const float scale2 = MOD ? 1.f : a.scale_log2 == 0.f ? 0x1p-126f : fabsf(a.scale_log2), slack = tree_slack(scale2);
 
     auto block = [&](int n, auto EDGE) {
         constexpr bool edge = decltype(EDGE)::value;
         typedef __attribute__((address_space(3))) uint8_t lds_u8;
+        // Of two workgroups on a CU the one that came first issues first, and would be done a quarter sooner (76 and 97 us of
+        // 8 x 8192 tokens, 64 drafted); the other one goes first in every second block (102.5 -> 99.0 us; a chain of
+        // 512 on 2 x 8192 164 -> 159).
+        if (cold.late()) {
+            if (n & 1) __builtin_amdgcn_s_setprio(1);
+            else __builtin_amdgcn_s_setprio(0);
+        }
         if (((n + 1) & 63) == 0 && n + 1 < o.n) load_ids(n + 1);
         issue(n + 1);
         lds_u8* const buf = (lds_u8*)S.block[0] + (n & 1) * (8 * kDecPageBytes);
@@ -978,34 +1059,21 @@ __device__ __forceinline__ void tree_piece_wide(TreeWideShared<NT>& S, const Tre
             }
         }
 
-        // Online softmax in base 2, as in tree_piece.
-        float mn[NT];
+        // Online softmax (tree_grow)
         bool grow = false;
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            float mx = x[t][0];
-#pragma unroll
-            for (int e = 1; e < 16; ++e) mx = fmaxf(mx, x[t][e]);
-            mn[t] = fmaxf(m[t], col4_reduce<true>(mx));
-            grow |= mn[t] > m[t];
-        }
+        for (int t = 0; t < NT; ++t) grow |= tree_largest<16>(x[t]) > m[t] + slack;
         if (__builtin_amdgcn_ballot_w64(grow)) {
 #pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                const float al = mn[t] > m[t] ? __builtin_amdgcn_exp2f((m[t] - mn[t]) * scale2) : 1.f;
-                l[t] *= al;
-#pragma unroll
-                for (int dt = 0; dt < 8; ++dt) acc[t][dt] *= al;
-                m[t] = mn[t];
-            }
+            for (int t = 0; t < NT; ++t) tree_grow(tree_largest<16>(x[t]), m[t], l[t], acc[t], scale2);
         }
         pf16x8 w[NT][2];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-            const float ms = m[t] == -INFINITY ? 0.f : m[t];
+            const float c = tree_offset(m[t], scale2);
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-                const float pe = __builtin_amdgcn_exp2f(fmaf(x[t][e] - ms, scale2, 15.f));
+                const float pe = __builtin_amdgcn_exp2f(fmaf(x[t][e], scale2, c));
                 l[t] += pe;
                 w[t][e >> 3][e & 7] = (_Float16)pe;
             }
@@ -1040,10 +1108,11 @@ __device__ __forceinline__ void tree_piece_wide(TreeWideShared<NT>& S, const Tre
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         u[i] &= keep[h][i];
-                        wild |= ((u[i] & 0x7C00u) == 0x7C00u) | ((u[i] & 0x7C000000u) == 0x7C000000u);
+                        wild |= tree_not_finite(u[i]);
                     }
                     va[dt & AHEAD][h] = __builtin_bit_cast(pf16x8, u);
                 }
+                wild = tree_fresh(wild);   // (now, or every element waits in a register for the last)
             }
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -1078,7 +1147,7 @@ __device__ __forceinline__ void tree_piece_wide(TreeWideShared<NT>& S, const Tre
         const int r = 16 * (4 * t + wave) + (int)(tree_fresh(lane) & 15u);
         if (r >= rows) continue;
         const float inv = L == 0.f ? 0.f : 1.f / L;
-        const float lse = L == 0.f ? -INFINITY : fmaf(m[t] == -INFINITY ? 0.f : m[t], scale2, __builtin_amdgcn_logf(L) - 15.f) * kTreeLn2;
+        const float lse = L == 0.f ? -INFINITY : fmaf(m[t] == -INFINITY ? 0.f : m[t], scale2, __builtin_amdgcn_logf(L) - kTreeShift) * kTreeLn2;
         if (slot < 0) {
             const int i = r / f.G;
             const size_t row = (size_t)(token0 + i) * f.Hq + kvh_ * f.G + (r - i * f.G);
@@ -1107,38 +1176,28 @@ __device__ __forceinline__ void tree_workgroup(const TreeArgs& a, Sh& S, Piece p
     PD_STAMP(0);
     const int g = blockIdx.x / a.Hkv, kvh = blockIdx.x - g * a.Hkv;
     if (threadIdx.x == 0) S.wild[0] = 0;
-    int64_t lo, hi, units;
-    int ranges;
-    const bool some = tree_find_range(a, S.scan, g, lo, hi, units, ranges);
-    if (!some) {
+    TreeRange r;
+    if (!tree_find_range(a, S.scan, g, r)) {
         if (kvh == 0 && threadIdx.x == 0) a.cuts[g] = make_int4(0, 0, 0, 0);
         return;
     }
+    PD_STAMP(1);
     // The first item, the units of it before the range, and (kv head 0) what the merge has to know: an item that
     // the boundary before this range cuts, which of its cuts that is, and its pieces.
-    PD_STAMP(1);
     const int lane = threadIdx.x & 63;
-    int b = __builtin_amdgcn_readfirstlane(S.scan.first), j, skip;
-    int left = __builtin_amdgcn_readfirstlane((int)(hi - lo));
-    // (the half of the entries' register that holds sequence b's)
-    const int after = tree_load_entry(*tree_args(), b + 1, lane);
-    int half = 0, entries = S.scan.tables[min(lane, 4)];
-    entries = lane < 8 ? entries : after;
+    int b = r.b, left = r.left, j, skip;
+    int half = 0, entries = r.entries;   // (the half of the entries that holds sequence b's)
     auto entry = [&](int i) { return __builtin_amdgcn_readlane(entries, half + i); };
-    auto sequence = [&](const auto& k) {
-        return tree_seq(entry(0), entry(1), entry(2), entry(3), entry(4), k.n_tokens, k.tpg, k.window, k.sink);
-    };
+    auto sequence = [&](const auto& k) { return tree_seq_of(k, entry(0), entry(1), entry(2), entry(3), entry(4)); };
     {
         const auto& k = *tree_args();
         const TreeSeq t = sequence(k);
-        const int64_t in = lo - tree_uniform(S.scan.prefix);
-        j = __builtin_amdgcn_readfirstlane((int)(in / t.units()));
-        skip = __builtin_amdgcn_readfirstlane((int)(in - (int64_t)j * t.units()));
+        j = __builtin_amdgcn_readfirstlane(t.group_of(r.in));
+        skip = __builtin_amdgcn_readfirstlane((int)(r.in - t.before(j)));
         if (kvh == 0 && threadIdx.x == 0) {
-            const int64_t first = lo - skip;
-            const int g0 = tree_range_of(units, ranges, first), g1 = tree_range_of(units, ranges, first + t.units() - 1);
-            const int i0 = j * k.tpg;
-            k.cuts[g] = make_int4(max(entry(3), 0) + i0, min(k.tpg, t.n - i0) * k.G, skip > 0 ? g1 - g0 + 1 : 0, g - g0 - 1);
+            const int64_t first = r.lo - skip;
+            const int g0 = r.cuts.of(first), g1 = r.cuts.of(first + t.units(j) - 1), i0 = j << k.tl;
+            k.cuts[g] = make_int4(max(entry(3), 0) + i0, min(1 << k.tl, t.n - i0) * k.G, skip > 0 ? g1 - g0 + 1 : 0, g - g0 - 1);
         }
     }
     int par = 0;
@@ -1156,14 +1215,14 @@ __device__ __forceinline__ void tree_workgroup(const TreeArgs& a, Sh& S, Piece p
             half ^= 8;
             continue;
         }
-        const int take = min(left, p.q.units() - skip);
-        p.i0 = j * k.tpg;
-        p.tokens = min(k.tpg, p.q.n - p.i0);
+        const int units = p.q.units(j), take = min(left, units - skip);
+        p.i0 = j << k.tl;
+        p.tokens = min(1 << k.tl, p.q.n - p.i0);
         p.rows = p.tokens * k.G;
         p.p0 = skip;
         p.p1 = min(skip + take, p.q.attended());
-        const int s = tree_slot(skip, take, p.q.units());
-        p.slot = s < 0 ? -1 : 2 * (int)blockIdx.x + s;
+        const int s = tree_slot(skip, take, units);
+        p.slot = s < 0 ? -1 : 2 * (int)tree_fresh_s(blockIdx.x) + s;
         p.par = par;
         left -= take;
         skip = 0;
@@ -1172,7 +1231,7 @@ __device__ __forceinline__ void tree_workgroup(const TreeArgs& a, Sh& S, Piece p
         // (the loop's own state is kept in lanes of the entries' register meanwhile)
         const uint32_t x = tree_fresh((uint32_t)lane);
         entries = x < 16 ? entries : x == 16 ? left : x == 17 ? b : x == 18 ? j : x == 19 ? half | par
-                : x == 20 ? p.i0 : x == 21 ? p.rows : x == 22 ? p.q0 : x == 23 ? p.slot : p.tokens;
+                : x == 20 ? p.i0 : x == 21 ? p.rows : x == 22 ? p.q0 : x == 23 ? p.slot : (int)((int)tree_fresh_s(blockIdx.x) * 2 >= k.ranges * k.Hkv);
         entries = (int)tree_fresh((uint32_t)entries);
         piece(p, kvh, entries);
         left = __builtin_amdgcn_readlane(entries, 16);
@@ -1205,25 +1264,32 @@ __global__ __launch_bounds__(kTreeThreads) void tree_merge_kernel(TreeArgs a, in
     const int4 cut = a.cuts[g];
     const int n = cut.z, g0 = g - 1 - cut.w;
     if (n == 0) return;
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, half = lane >> 5, c = lane & 31;
-    for (int r = cut.w + (n - 1) * (int)(blockIdx.y * kTreeWaves + wave); r < cut.y; r += (n - 1) * (int)gridDim.y * kTreeWaves) {
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, c = lane & 31;
+    __shared__ float s_m[8], s_w[8];
+    __shared__ pf32x4 s_o[8][32];
+    // Few pieces: a row per wave, its two halves taking every second piece. Many: a row at a time, eight halves.
+    const bool many = n > 8;
+    const int halves = many ? 8 : 2, half = many ? tid >> 5 : lane >> 5;
+    const int step = many ? (int)gridDim.y : (int)gridDim.y * kTreeWaves, at = many ? (int)blockIdx.y : (int)blockIdx.y * kTreeWaves + wave;
+    for (int x = at; cut.w + (n - 1) * x < cut.y; x += step) {
+        const int r = cut.w + (n - 1) * x;
         // piece k: range g0 + k, slot 1 of the first's workgroup, slot 0 of the others'
         auto slot = [&](int k) { return ((size_t)((g0 + k) * a.Hkv + kvh) * 2 + (k == 0)) * ROWS + r; };
         float m = -INFINITY, ws = 0.f;
         pf32x4 o = pf32x4{0.f, 0.f, 0.f, 0.f};
         constexpr int U = 4;
-        for (int k0 = half; k0 - half < n; k0 += 2 * U) {
+        for (int k0 = half; k0 - half < n; k0 += halves * U) {
             float l[U];
             pf32x4 v[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const size_t s = slot(min(k0 + 2 * u, n - 1));
+                const size_t s = slot(min(k0 + halves * u, n - 1));
                 l[u] = a.part_lse[s];
                 v[u] = *reinterpret_cast<const pf32x4*>(a.part_o + s * kHeadDim + 4 * c);
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                if (k0 + 2 * u >= n || l[u] == -INFINITY) continue;
+                if (k0 + halves * u >= n || l[u] == -INFINITY) continue;
                 const float mn = fmaxf(m, l[u]);
                 const float sc = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - mn) * kTreeLog2e);
                 const float w = __builtin_amdgcn_exp2f((l[u] - mn) * kTreeLog2e);
@@ -1233,23 +1299,43 @@ __global__ __launch_bounds__(kTreeThreads) void tree_merge_kernel(TreeArgs a, in
                 m = mn;
             }
         }
-        const float m2 = __shfl_xor(m, 32, 64), ws2 = __shfl_xor(ws, 32, 64), M = fmaxf(m, m2);
-        const float s1 = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - M) * kTreeLog2e);
-        const float s2 = m2 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m2 - M) * kTreeLog2e);
-        // (the lower half's pieces first, in both)
-        const float W = half == 0 ? ws * s1 + ws2 * s2 : ws2 * s2 + ws * s1;
-        const float inv = W == 0.f ? 0.f : 1.f / W;
-        pf16x4 h;
+        // The halves' states, weighted to the largest maximum and added in the halves' order
+        float M = m, W = 0.f;
+        pf32x4 O = pf32x4{0.f, 0.f, 0.f, 0.f};
+        auto add = [&](float hm, float hw, const pf32x4& ho) {
+            const float s = hm == -INFINITY ? (hw == 0.f ? 0.f : hw) : __builtin_amdgcn_exp2f((hm - M) * kTreeLog2e);   // (hw: NaN)
+            W = fmaf(hw, s, W);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float o2 = __shfl_xor(o[j], 32, 64);
-            h[j] = (_Float16)((o[j] * s1 + o2 * s2) * inv);
+            for (int j = 0; j < 4; ++j) O[j] = fmaf(ho[j], s, O[j]);
+        };
+        if (many) {   // (uniform over the workgroup, as the loop is)
+            if (c == 0) {
+                s_m[half] = m;
+                s_w[half] = ws;
+            }
+            s_o[half][c] = o;
+            __syncthreads();
+#pragma unroll
+            for (int h = 0; h < 8; ++h) M = fmaxf(M, s_m[h]);
+#pragma unroll
+            for (int h = 0; h < 8; ++h) add(s_m[h], s_w[h], s_o[h][c]);
+            __syncthreads();
+        } else {
+            const float m2 = __shfl_xor(m, 32, 64), w2 = __shfl_xor(ws, 32, 64);
+            pf32x4 o2;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o2[j] = __shfl_xor(o[j], 32, 64);
+            M = fmaxf(M, m2);
+            add(m, ws, o);   // (written by the lower half, whose own comes first)
+            add(m2, w2, o2);
         }
         if (half == 0) {
+            const float inv = W == 0.f ? 0.f : 1.f / W;
             const int i = r / a.G;
             const size_t row = (size_t)(cut.x + i) * a.Hq + kvh * a.G + (r - i * a.G);
-            *reinterpret_cast<pf16x4*>(a.out + row * kHeadDim + 4 * c) = h;
-            if (c == 0) a.lse[row] = W == 0.f ? -INFINITY : m == -INFINITY && m2 == -INFINITY ? W : M + __builtin_amdgcn_logf(W) * kTreeLn2;
+            *reinterpret_cast<pf16x4*>(a.out + row * kHeadDim + 4 * c) =
+                pf16x4{(_Float16)(O[0] * inv), (_Float16)(O[1] * inv), (_Float16)(O[2] * inv), (_Float16)(O[3] * inv)};
+            if (c == 0) a.lse[row] = W == 0.f ? -INFINITY : fmaf(__builtin_amdgcn_logf(W), kTreeLn2, M == -INFINITY ? 0.f : M);
         }
     }
 }

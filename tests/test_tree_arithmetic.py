@@ -17,17 +17,21 @@ def arith(tmp_path_factory):
     subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Werror", "-shared", "-fPIC",
                     os.path.join(ROOT, "tests", "cpp", "tree_arith.cpp"), "-o", so], check=True)
     lib = ctypes.CDLL(so)
-    lib.t_start.restype = ctypes.c_longlong
-    lib.t_start.argtypes = [ctypes.c_longlong, ctypes.c_int, ctypes.c_int]
-    lib.t_ranges.argtypes = [ctypes.c_longlong, ctypes.c_int, ctypes.c_int]
-    lib.t_of.argtypes = [ctypes.c_longlong, ctypes.c_int, ctypes.c_longlong]
+    L, I = ctypes.c_longlong, ctypes.c_int
+    lib.t_ranges.argtypes, lib.t_start.argtypes, lib.t_of.argtypes = [L, I, I, I, I], [L, I, I, I, I, I], [L, I, I, I, I, L]
+    lib.t_start.restype = lib.t_before.restype = L
+    lib.t_group.argtypes = [ctypes.c_void_p, L]
     return lib
 
 
+def _args(*args):
+    return (ctypes.c_int * 10)(*args)
+
+
 def _seq(lib, *args):
-    out = (ctypes.c_int * 9)()
-    lib.t_seq(*args, out)
-    return dict(zip(("len", "n", "ctx", "np", "s", "w0", "groups", "attended", "units"), out))
+    out = (ctypes.c_int * 8)()
+    lib.t_seq(_args(*args), out)
+    return dict(zip(("len", "n", "ctx", "np", "s", "w0", "groups", "attended"), out))
 
 
 @pytest.mark.parametrize("seed", range(30))
@@ -37,13 +41,17 @@ def test_ranges_cover_every_unit_once(arith, seed):
     units = sum(g * u for g, u in items)
     if units == 0:
         return
-    most, least = int(rng.choice([1, 2, 7, 64, 500])), int(rng.choice([1, 4, 8]))
-    R = arith.t_ranges(units, most, least)
+    most, least = int(rng.choice([1, 2, 7, 64, 500])), int(rng.choice([4, 8]))
+    early, late = [(1, 1), (9, 7), (5, 3), (8, 7)][int(rng.integers(0, 4))]
+    cut = (units, most, least, early, late)
+    R = arith.t_ranges(*cut)
     assert 1 <= R <= max(1, most) and (R == 1 or units >= R * least)
-    starts = [arith.t_start(units, R, g) for g in range(R + 1)]
+    starts = [arith.t_start(*cut, g) for g in range(R + 1)]
     assert starts[0] == 0 and starts[-1] == units and all(a < b for a, b in zip(starts, starts[1:]))
+    if R == most and R > 1 and R % 2 == 0:
+        assert abs(starts[R // 2] * late - (units - starts[R // 2]) * early) <= early + late
     for x in rng.integers(0, units, 50):
-        g = arith.t_of(units, R, int(x))
+        g = arith.t_of(*cut, int(x))
         assert starts[g] <= x < starts[g + 1]
     # walk the ranges as the kernel does, and note who writes what of which item
     flat = [(i, j, u) for i, (g, u) in enumerate(items) for j in range(g)]
@@ -52,10 +60,10 @@ def test_ranges_cover_every_unit_once(arith, seed):
     for g in range(R):
         k = int(np.searchsorted(firsts, starts[g], side="right")) - 1
         skip, left = int(starts[g] - firsts[k]), starts[g + 1] - starts[g]
-        g0, g1 = arith.t_of(units, R, int(firsts[k])), arith.t_of(units, R, int(firsts[k + 1]) - 1)
-        if skip > 0 and g0 == g - 1:
-            assert k not in merges
-            merges[k] = [(g0 + i, 1 if i == 0 else 0) for i in range(g1 - g0 + 1)]
+        g0, g1 = arith.t_of(*cut, int(firsts[k])), arith.t_of(*cut, int(firsts[k + 1]) - 1)
+        if skip > 0:   # every cut of an item knows them all
+            mine = [(g0 + i, 1 if i == 0 else 0) for i in range(g1 - g0 + 1)]
+            assert g0 < g <= g1 and merges.setdefault(k, mine) == mine
         while left > 0:
             u = flat[k][2]
             take = min(left, u - skip)
@@ -77,8 +85,11 @@ def test_ranges_cover_every_unit_once(arith, seed):
 
 
 def test_large_batches_stay_in_range(arith):
-    units, R = 9_000_000_000, 512
-    assert arith.t_start(units, R, 511) == units * 511 // 512 and arith.t_of(units, R, units - 1) == 511
+    cut = (9_000_000_000, 512, 8, 9, 7)
+    starts = [arith.t_start(*cut, g) for g in range(513)]
+    assert starts == [cut[0] * (9 * min(g, 256) + 7 * max(g - 256, 0)) // 4096 for g in range(513)]
+    for g in range(512):
+        assert arith.t_of(*cut, starts[g]) == g and arith.t_of(*cut, starts[g + 1] - 1) == g
 
 
 @pytest.mark.parametrize("seed", range(40))
@@ -88,23 +99,35 @@ def test_attended_pages_hold_every_key_in_a_window(arith, seed):
     n = min(n, length)
     window, sink = int(rng.choice([0, 1, 5, 16, 40, 300])), int(rng.choice([0, 1, 16, 17, 64, 500]))
     np_, last = -(-length // 16), (length - 1) % 16 + 1
-    args = (7, 7 + np_, last, 3, 3 + n, 100, int(rng.choice([2, 4, 16])), window, sink)
+    args = (7, 7 + np_, last, 3, 3 + n, 100, int(rng.choice([2, 4, 16, 64])), window, sink, int(rng.integers(0, 2)))
     t = _seq(arith, *args)
+    tpg, args = args[6], _args(*args)
     assert (t["len"], t["n"], t["ctx"], t["np"]) == (length, n, length - n, np_)
-    assert t["groups"] == -(-n // args[6])
-    pages = [arith.t_page(*args, i) for i in range(t["attended"])]
+    assert t["groups"] == -(-n // tpg)
+    pages = [arith.t_page(args, i) for i in range(t["attended"])]
     assert pages == sorted(set(pages)) and pages[-1] == np_ - 1
     for pos in range(n):   # any position a token may have: ctx + a depth of 0 or more
         seen = [k for k in range(length) if window == 0 or k >= t["ctx"] + pos - window + 1 or k < sink]
         assert {k // 16 for k in seen} <= set(pages)
     for page in range(np_ + 1):
-        assert arith.t_below(*args, page) == sum(x < page for x in pages)
+        assert arith.t_below(args, page) == sum(x < page for x in pages)
+    # the units of every group: enough for all the pages that its tokens may see, and found again from the sum
+    start = 0
+    for j in range(t["groups"]):
+        u = arith.t_units(args, j)
+        assert u >= 1 and arith.t_before(args, j) == start
+        last_key = t["ctx"] + min(n, (j + 1) * tpg) - 1 if args[9] and 2 * n > t["ctx"] else length - 1
+        assert u >= sum(p <= last_key // 16 for p in pages)
+        for x in (start, start + u // 2, start + u - 1):
+            assert arith.t_group(args, x) == j
+        start += u
+    assert arith.t_before(args, t["groups"]) == start
     if window and t["ctx"] > window + sink + 64:
         assert len(pages) < np_
 
 
 @pytest.mark.parametrize("args,expect", [
-    ((5, 5, 0, 0, 4, 10, 4, 0, 0), dict(len=0, n=4, ctx=-4, np=0, groups=1, attended=0, units=1)),
+    ((5, 5, 0, 0, 4, 10, 4, 0, 0), dict(len=0, n=4, ctx=-4, np=0, groups=1, attended=0)),
     ((5, 3, 9, 0, 4, 10, 4, 0, 0), dict(len=0, np=0)),                       # a page table that goes back
     ((0, 2, 99, 0, 4, 10, 4, 0, 0), dict(len=32)), ((0, 2, -3, 0, 4, 10, 4, 0, 0), dict(len=17)),
     ((0, 2, 5, 4, 2, 10, 4, 0, 0), dict(n=0, groups=0)),                     # and tokens that do
@@ -112,8 +135,10 @@ def test_attended_pages_hold_every_key_in_a_window(arith, seed):
     ((0, 1, 3, 0, 9, 10, 4, 8, 2 ** 31 - 1), dict(len=3, n=9, ctx=-6, s=0, w0=0, attended=1)),
 ])
 def test_tables_that_make_no_sense(arith, args, expect):
-    t = _seq(arith, *args)
-    assert {k: t[k] for k in expect} == expect
+    for causal in (0, 1):
+        t = _seq(arith, *args, causal)
+        assert {k: t[k] for k in expect} == expect
+        assert all(arith.t_units(_args(*args, causal), j) >= 1 for j in range(t["groups"]))
 
 
 @pytest.mark.parametrize("step,width", [(8, 2), (4, 4)])
@@ -132,3 +157,16 @@ def test_order_of_blocks(arith, step, width):
         assert sorted(order[:plain]) == want
         plain_seen += plain
     assert plain_seen > 1000
+
+
+@pytest.mark.parametrize("tpg", [2, 4, 8, 16, 32, 128])
+def test_units_of_a_long_chain(arith, tpg):
+    """A chunk of a prefill: later groups see more pages, and the sum says so."""
+    args = _args(0, 100, 16, 0, 1500, 1500, tpg, 0, 0, 1)   # 1600 cached, 100 of them before the chunk
+    groups = -(-1500 // tpg)
+    units = [arith.t_units(args, j) for j in range(groups)]
+    need = [-(-(100 + min(1500, (j + 1) * tpg)) // 16) for j in range(groups)]
+    assert all(n <= u <= n + max(1, tpg // 16) for n, u in zip(need, units))
+    assert [arith.t_before(args, j) for j in range(groups + 1)] == np.concatenate([[0], np.cumsum(units)]).tolist()
+    for x in range(0, sum(units), 7):
+        assert arith.t_group(args, x) == int(np.searchsorted(np.cumsum(units), x, side="right"))
