@@ -176,7 +176,7 @@ struct RopeArgs {
     int64_t        q_stride, k_stride, v_stride;   // bytes
     int            n, B, Hq, Hkv, rotary_dim, interleaved;
     float          scale;
-    int            tpb;           // tokens per workgroup, and the multiplier of a token's rows (set by the launch)
+    int            tpb, rows_wg;  // tokens and rows per workgroup, and the multiplier of a token's rows (set by the launch)
     uint32_t       rows_m;
 };
 

@@ -15,9 +15,18 @@
 
 namespace pdattn {
 
-// x / d for x >= 0, d > 0: in 32 bits where they hold x (a 64-bit division is some hundred instructions).
-PD_RANGE_FN int64_t tree_div(int64_t x, int64_t d) {
-    return (uint64_t)x >> 32 || (uint64_t)d >> 32 ? x / d : (int64_t)((uint32_t)x / (uint32_t)d);
+// x / d for x >= 0, 0 < d < 2^16, in 32 bits (a 64-bit division is some hundred instructions).
+PD_RANGE_FN int64_t tree_div(int64_t x, uint32_t d) {
+    const uint64_t u = (uint64_t)x;
+    if (u >> 32 == 0) return (int64_t)((uint32_t)u / d);
+    uint64_t q = 0;
+    uint32_t rest = 0;
+    for (int i = 48; i >= 0; i -= 16) {
+        rest = rest << 16 | (uint32_t)(u >> i & 0xFFFF);
+        q = q << 16 | rest / d;
+        rest %= d;
+    }
+    return (int64_t)q;
 }
 
 // One sequence of the batch as the kernels see it. Positions count from the sequence's first cached token.
@@ -44,7 +53,6 @@ struct TreeSeq {
     // the group that holds the sequence's unit x
     PD_RANGE_FN int group_of(int64_t x) const {
         if (groups <= 1) return 0;
-        if (st == 0) return (int)tree_div(x, u0);
         int lo = 0, hi = groups - 1;
         while (lo < hi) {
             const int mid = (lo + hi + 1) / 2;
@@ -114,27 +122,33 @@ PD_RANGE_FN TreeOrder tree_order(int first, int step, int width, int p1, int a0,
 // one that came first issues first: where all `most` ranges are used, the first half of them is longer, `early` to
 // `late`.
 struct TreeCuts {
-    int64_t units;
-    int ranges, early, late, half, total;   // half: ranges of the first kind; total: the sum of their weights
-    PD_RANGE_FN int64_t start(int g) const {
+    int64_t step;                           // units = step total + rest
+    int rest;
+    int ranges, early, late, half, total;   // half: ranges of the first kind; total: the sum of their weights, below 2^15
+    PD_RANGE_FN int64_t start(int g) const {   // units w / total
         const int w = g <= half ? early * g : early * half + late * (g - half);
-        return tree_div(units * w, total);
+        return step * w + (uint32_t)rest * (uint32_t)w / (uint32_t)total;
     }
-    // the range that holds unit x
+    // the range that holds unit x: a guess in 32-bit floats, put right
     PD_RANGE_FN int of(int64_t x) const {
-        const int y = (int)tree_div((x + 1) * total - 1, units);
-        return y < early * half ? (int)((uint32_t)y / (uint32_t)early) : half + (int)((uint32_t)(y - early * half) / (uint32_t)late);
+        const float y = (float)x / ((float)step + (float)rest / (float)total), e = (float)(early * half);
+        int g = (int)(y < e ? y / (float)early : (float)half + (y - e) / (float)late);
+        g = g < 0 ? 0 : g >= ranges ? ranges - 1 : g;
+        while (g > 0 && start(g) > x) --g;
+        while (g + 1 < ranges && start(g + 1) <= x) ++g;
+        return g;
     }
 };
 PD_RANGE_FN TreeCuts tree_cuts(int64_t units, int most, int least, int early, int late) {
     TreeCuts c;
-    c.units = units;
-    const int64_t r = tree_div(units, least);
+    const int64_t r = tree_div(units, (uint32_t)least);
     c.ranges = units <= 0 ? 0 : r < 1 ? 1 : r > most ? most : (int)r;
     c.half = c.ranges == most ? most / 2 : 0;
     c.early = early;
     c.late = c.half > 0 ? late : 1;
     c.total = c.half > 0 ? early * c.half + late * (c.ranges - c.half) : c.ranges;
+    c.step = c.total > 0 ? tree_div(units, (uint32_t)c.total) : 0;
+    c.rest = (int)(units - c.step * c.total);
     return c;
 }
 
