@@ -1655,9 +1655,12 @@ int tree_layout(const pdattn_tree_params* p, int G, TreeLayout* L) {
     const bool plain = !(p->score.soft_cap > 0.f) && !p->score.slopes && p->score.window <= 0;
     const bool many = plain && rows > 128 && (int64_t)p->n_tokens * G > (int64_t)128 * p->B;
     L->rows = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : many ? 256 : 128;
-    L->ranges = std::max(1, (L->rows == 256 ? 1 : 2) * f.cus / p->Hkv);   // (workgroups that a CU holds)
-    const size_t slots = (size_t)2 * L->ranges * p->Hkv * L->rows;
-    size_t off = align_up(sizeof(int4) * L->ranges);
+    const int two = std::max(1, 2 * f.cus / p->Hkv);   // (workgroups that the CUs hold)
+    L->ranges = L->rows == 256 ? std::max(1, f.cus / p->Hkv) : two;
+    // (the same bytes with 128 rows and with 256, so that the scores do not matter to them)
+    const int64_t most = L->rows < 128 ? (int64_t)two * L->rows : std::max<int64_t>((int64_t)two * 128, rows > 128 ? std::max(1, f.cus / p->Hkv) * (int64_t)256 : 0);
+    const size_t slots = (size_t)2 * most * p->Hkv;
+    size_t off = align_up(sizeof(int4) * two);
     L->off_plse = off; off += align_up(sizeof(float) * slots);
     L->off_po = off;   off += align_up(sizeof(float) * slots * kHeadDim);
     L->bytes = off;

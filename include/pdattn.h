@@ -460,7 +460,7 @@ typedef struct pdattn_tree_params {
 } pdattn_tree_params;
 
 /* Workspace bytes pdattn_tree_attention needs for `p` (0 on an invalid `p`). They depend on the device
- * and on B, Hq, Hkv, n_tokens and max_tokens alone. */
+ * and on B, Hq, Hkv, n_tokens, max_tokens and whether q_indptr is NULL alone. */
 size_t pdattn_tree_workspace_size(const pdattn_tree_params* p);
 /* out [n_tokens, Hq, 128] fp16 and lse [n_tokens, Hq] fp32; the workspace as in
  * pdattn_decode_attention. */

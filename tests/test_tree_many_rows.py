@@ -156,3 +156,23 @@ def test_two_streams_with_their_own_workspaces():
     for dd, ref, ws in zip(dds, refs, wss):
         check_attention(dd.out.float().cpu().numpy(), dd.lse.cpu().numpy(), ref, "two streams")
         pdattn.workspace_release(ws)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("Hq,Hkv,new", [(8, 2, 64), (8, 2, 20), (16, 2, 33), (4, 4, 5), (1200, 300, 50)])
+def test_the_scores_do_not_change_the_workspace(Hq, Hkv, new):
+    """A workspace sized for plain scores serves changed ones, masks and chains, and a graph of either."""
+    base = dict(B=2, Hq=Hq, Hkv=Hkv, n_tokens=2 * new, q_indptr=1 << 20, max_tokens=new)
+    ptrs = [1 << 20] * 6
+    sizes = {pdattn.tree_workspace_size(pdattn.make_tree_params(*ptrs, **base, **kw))
+             for kw in (dict(), dict(soft_cap=5.0), dict(window=50), dict(slopes=1 << 20), dict(mask=1 << 20, mask_words=2))}
+    assert len(sizes) == 1 and min(sizes) > 0
+    if Hkv > 4:
+        return
+    dr = make_draft([100, 400], [new, new], Hq, Hkv, seed=61)
+    mem = torch.empty(min(sizes), dtype=torch.uint8, device="cuda")
+    ws, dd = pdattn.Workspace(mem.data_ptr(), mem.numel(), 0), DeviceDraft(dr)
+    for kw in (dict(), dict(soft_cap=5.0, window=70)):
+        pdattn.tree_attention(dd.params(**kw), dd.out, dd.lse, ws)
+        torch.cuda.synchronize()
+        check_attention(dd.out.float().cpu().numpy(), dd.lse.cpu().numpy(), oracle_attention(dr, **kw), f"scores {kw}")
