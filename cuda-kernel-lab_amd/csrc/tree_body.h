@@ -448,14 +448,14 @@ __device__ __forceinline__ void tree_cap(float (&x)[NT][N]) {
 
 // The distance bias of keys that every row sees: x[t][4 y + j] is of key first[y] + j (relative to the context; the lane's
 // four of a page).
-template <bool MOD, int NT, int T>
-__device__ __forceinline__ void tree_bias(float (&x)[NT][4 * T], const int (&first)[T], const TreeRows<NT>& R) {
+template <bool MOD, int NA, int NT, int T>
+__device__ __forceinline__ void tree_bias(float (&x)[NA][4 * T], const int (&first)[T], const TreeRows<NT>& R) {
     if constexpr (MOD) {
         if (tree_args()->slopes == nullptr) return;
 #pragma unroll
         for (int y = 0; y < T; ++y)
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
+            for (int t = 0; t < NA; ++t)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) x[t][4 * y + j] = fmaf(R.slope[t], (float)(first[y] + j - R.pos[t]), x[t][4 * y + j]);
     }
@@ -554,14 +554,14 @@ __device__ __forceinline__ float tree_largest(const float (&x)[N]) {
 }
 // The lag in scores (finite: -infinity plus it stays).
 __device__ __forceinline__ float tree_slack(float scale2) { return fminf(kTreeLag / scale2, 1e38f); }
-template <int NT, int N>
-__device__ __forceinline__ void tree_softmax(const float (&x)[NT][N], TreeState<NT>& st, pf16x8 (&w)[NT][N / 8], float scale2, float slack) {
+template <int NA, int NT, int N>
+__device__ __forceinline__ void tree_softmax(const float (&x)[NA][N], TreeState<NT>& st, pf16x8 (&w)[NA][N / 8], float scale2, float slack) {
     bool grow = false;
 #pragma unroll
-    for (int t = 0; t < NT; ++t) grow |= tree_largest(x[t]) > st.m[t] + slack;
+    for (int t = 0; t < NA; ++t) grow |= tree_largest(x[t]) > st.m[t] + slack;
     if (__builtin_amdgcn_ballot_w64(grow)) {
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
+        for (int t = 0; t < NA; ++t) {
             const float mn = fmaxf(st.m[t], col4_reduce<true>(tree_largest(x[t])));
             const float al = mn > st.m[t] ? __builtin_amdgcn_exp2f((st.m[t] - mn) * scale2) : 1.f;
             st.l[t] *= al;
@@ -571,7 +571,7 @@ __device__ __forceinline__ void tree_softmax(const float (&x)[NT][N], TreeState<
         }
     }
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
+    for (int t = 0; t < NA; ++t) {
         const float c = st.m[t] == -INFINITY ? kTreeShift : fmaf(-st.m[t], scale2, kTreeShift);
 #pragma unroll
         for (int e = 0; e < N; ++e) {
@@ -975,7 +975,8 @@ __device__ __forceinline__ void tree_piece_wide(TreeWideShared<NW, NT>& S, const
     auto buffer = [&](int n) { return (lds_u8*)S.block[0] + (n & (NB - 1)) * kTreeBlockBytes; };
     // S^T: x[t][4 tk + j] = product of key 16 tk + 4 lg + j and row l16 of tile t; K of tile tk + 1 is read before the MFMAs
     // of tile tk (but in an edge block, whose bits take the registers)
-    auto scores = [&](int n, float (&x)[NT][16], auto EDGE) {
+    auto scores = [&](int n, auto& x, auto EDGE) {
+        constexpr int NA = sizeof(x) / sizeof(x[0]);
         constexpr int ahead = decltype(EDGE)::value ? 0 : 1;
         lds_u8* const buf = buffer(n);
         const uint32_t kl = tree_fresh((uint32_t)(l16 * 256 + ((((l16 >> 2) << 2) | (lg ^ (l16 & 3))) << 4)));
@@ -992,7 +993,7 @@ __device__ __forceinline__ void tree_piece_wide(TreeWideShared<NW, NT>& S, const
             if (tk < 4 - ahead) kfrag(tk + ahead, ka[(tk + ahead) & ahead]);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int t = 0; t < NT; ++t) {
+            for (int t = 0; t < NA; ++t) {
                 pf32x4 c = pf32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int ks = 0; ks < 4; ++ks) c = mfma16x16x32(ka[tk & ahead][ks], R.q[t][ks], c);
@@ -1007,7 +1008,7 @@ __device__ __forceinline__ void tree_piece_wide(TreeWideShared<NW, NT>& S, const
         return at < p1 ? sq.page(at) * kPage : end;
     };
     // Products to weights
-    auto weights = [&](int n, float (&x)[NT][16], pf16x8 (&w)[NT][2], auto EDGE) {
+    auto weights = [&](int n, auto& x, auto& w, auto EDGE) {
         tree_cap<MOD>(x);
         const int lg4 = (int)(tree_fresh(lane) >> 4) * 4;
         int first[4];
@@ -1023,7 +1024,8 @@ __device__ __forceinline__ void tree_piece_wide(TreeWideShared<NW, NT>& S, const
         tree_softmax(x, st, w, scale2, slack);
     };
     // O^T += V^T P^T; V of dim tile dt + 1 is read before the MFMAs of dt (but in an edge block)
-    auto product = [&](int n, const pf16x8 (&w)[NT][2], auto EDGE) {
+    auto product = [&](int n, const auto& w, auto EDGE) {
+        constexpr int NA = sizeof(w) / sizeof(w[0]);
         constexpr bool edge = decltype(EDGE)::value;
         constexpr int ahead = edge ? 0 : 1;
         lds_u8* const buf = buffer(n) + kTreeBlockBytes / 2;
@@ -1062,7 +1064,7 @@ __device__ __forceinline__ void tree_piece_wide(TreeWideShared<NW, NT>& S, const
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int t = 0; t < NT; ++t) st.acc[t][dt] = mfma16x16x32(va[dt & ahead][h], w[t][h], st.acc[t][dt]);
+                for (int t = 0; t < NA; ++t) st.acc[t][dt] = mfma16x16x32(va[dt & ahead][h], w[t][h], st.acc[t][dt]);
             __builtin_amdgcn_sched_barrier(0);
         }
     };
@@ -1071,7 +1073,8 @@ __device__ __forceinline__ void tree_piece_wide(TreeWideShared<NW, NT>& S, const
     __syncthreads();   // mask rows, depths, the first block
     PD_STAMP(4 + 8 * cold.flag());
     if constexpr (NW == 4) {
-        auto block = [&](int n, auto EDGE) {
+        auto block = [&](int n, auto EDGE, auto TILES) {
+            constexpr int NA = decltype(TILES)::value;
             // Of two workgroups on a CU the one that came first issues first, and would be done a quarter sooner (76 and 97
             // us of 8 x 8192 tokens, 64 drafted); the other one goes first in every second block (102.5 -> 99.0 us; a
             // chain of 512 on 2 x 8192 164 -> 159).
@@ -1080,16 +1083,25 @@ __device__ __forceinline__ void tree_piece_wide(TreeWideShared<NW, NT>& S, const
                 else __builtin_amdgcn_s_setprio(0);
             }
             issue(n + 1);
-            float x[NT][16];
-            pf16x8 w[NT][2];
+            float x[NA][16];
+            pf16x8 w[NA][2];
             scores(n, x, EDGE);
             weights(n, x, w, EDGE);
             product(n, w, EDGE);
             arrived(n + 1);
             dec_barrier();
         };
-        for (int n = 0; n < o.plain; ++n) block(n, std::false_type{});
-        for (int n = o.plain; n < o.n; ++n) block(n, std::true_type{});
+        // A wave whose second tile has no row leaves it out (32 ragged contexts, 5-27 drafted tokens at G = 8, so groups of
+        // 8-128 rows: 77.7 -> 75.0 us)
+        const std::integral_constant<int, NT> all{};
+        const std::integral_constant<int, 1> one{};
+        int n = 0;
+        if (NT == 1 || cold.rows() > 16 * (NW + wave)) {
+            for (; n < o.plain; ++n) block(n, std::false_type{}, all);
+        } else {
+            for (; n < o.plain; ++n) block(n, std::false_type{}, one);
+        }
+        for (; n < o.n; ++n) block(n, std::true_type{}, all);
     } else if (o.n > 0) {
         // Steps 0 .. n: the step in which both of a wave's blocks are plain is the loop; the others are the general one.
         const std::false_type plain{};
