@@ -1717,7 +1717,13 @@ int pdattn_tree_attention(const pdattn_tree_params* p, void* out, float* lse, pd
     a.rows = L.rows;
     a.tl = __builtin_ctz((unsigned)(L.rows / G));   // (both powers of two)
     a.ranges = L.ranges;
-    a.least_units = 8;
+    // What a range costs besides its pages: the start of a piece about two blocks' time. Ragged contexts of 200-6000 tokens, 32
+    // sequences: 5-27 drafted tokens at G = 8 75.8 us without, 69.8, 63.1, 64.4, 63.7 with 4, 8, 12, 16 pages; one token each 48.1
+    // without, 46.3, 46.1, 46.3, 46.0. With 128 rows, whose waves may leave out half, a page of a short group counts less:
+    // blocks of 64 keys took 2.05 us there, 2.74 with all rows.
+    a.weight = L.rows == 128 ? 4 : 1;
+    a.extra = a.weight * (L.rows <= 32 ? 16 : 8);
+    a.least_units = a.weight * 8;
     a.early = L.rows <= 32 ? 9 : 1;
     a.late = L.rows <= 32 ? 8 : 1;
     a.window = std::min(p->score.window, 1 << 30);   // (past any position: sums of positions fit an int)

@@ -215,6 +215,7 @@ struct TreeArgs {
     int rows, tl;                 // rows of a workgroup; 2^tl tokens of a group: rows / G
     int ranges, least_units;      // ranges of the grid, and units that a range has at least
     int early, late;              // lengths of the first half of the ranges to the others'
+    int weight, extra;            // units of a page and of an item's start (tree_seq)
     float scale_log2;             // sm_scale log2(e)
     float cap_in, cap_out;        // sm_scale / cap and cap log2(e), or 0
 };

@@ -3,10 +3,11 @@
 //
 // The rows of a sequence for one kv head (its n tokens times the G query heads of the head, a token's heads
 // together) are cut into groups of as many tokens as fill a workgroup's rows. Each (sequence, group) is an item; its
-// units are the pages that its tokens may see. The units of all items, in the order of sequences, groups and pages, are
-// cut into ranges, and workgroup (g, kv head) takes range g: pieces of items, one after the other. An item inside one
-// range is written by its workgroup. Of an item cut by range boundaries, the piece that starts it goes to partial
-// slot 2 w + 1 of its workgroup w = g Hkv + kv head, every later piece to slot 2 w of its.
+// units are `extra` for its start and `weight` for each page that its tokens may see. The units of all items, in the order of
+// sequences, groups and pages, are cut into ranges, and workgroup (g, kv head) takes range g: pieces of items, one after
+// the other; a page belongs to the range that holds its first unit. An item inside one range is written by its
+// workgroup. Of an item cut by range boundaries, the piece that starts it goes to partial slot 2 w + 1 of its
+// workgroup w = g Hkv + kv head, every later piece to slot 2 w of its.
 #pragma once
 
 #include <cstdint>
@@ -35,19 +36,32 @@ struct TreeSeq {
     int np;              // pages
     int s, w0;           // attended pages: [0, s) and [w0, np)
     int groups;
-    // units of group j: u0 + st (j >> cl). Chains: later tokens see more pages, a page more every 16 tokens.
+    // pages of group j: u0 + st (j >> cl). Chains: later tokens see more pages, a page more every 16 tokens.
     int u0, st, cl;
+    int wt, wl;          // units of a page of a group, and of the last group
+    int extra;           // units of a group's start
     PD_RANGE_FN int attended() const { return s + np - w0; }
     // the page at place i of the attended ones
     PD_RANGE_FN int page(int i) const { return i < s ? i : i - s + w0; }
     // the places of pages below page p (those before it in the order of places)
     PD_RANGE_FN int below(int p) const { return p <= s ? p : p <= w0 ? s : s + p - w0; }
-    PD_RANGE_FN int units(int j) const { return u0 + st * (j >> cl); }
+    PD_RANGE_FN int weight(int j) const { return j == groups - 1 ? wl : wt; }
+    PD_RANGE_FN int pages(int j) const { return u0 + st * (j >> cl); }
+    PD_RANGE_FN int units(int j) const { return pages(j) * weight(j) + extra; }
+    // the first page of group j whose first unit is x or later
+    PD_RANGE_FN int first_page(int j, int x) const {
+        const int k = weight(j), y = x - extra;
+        return y <= 0 ? 0 : k == 1 ? y : (int)(((uint32_t)y + (uint32_t)k - 1u) / (uint32_t)k);
+    }
+    // the first unit of the last page of group j
+    PD_RANGE_FN int last_unit(int j) const { return extra + (pages(j) - 1) * weight(j); }
     // units of the groups before j
     PD_RANGE_FN int64_t before(int j) const {
-        if (st == 0) return (int64_t)u0 * j;
         const int64_t m = j >> cl;
-        return (int64_t)u0 * j + st * ((m * (m - 1) / 2 << cl) + (j - (m << cl)) * m);
+        int64_t sum = (int64_t)u0 * j;
+        if (st) sum += st * ((m * (m - 1) / 2 << cl) + (j - (m << cl)) * m);
+        sum = sum * wt + (int64_t)extra * j;
+        return j == groups && j > 0 ? sum - (int64_t)pages(j - 1) * (wt - wl) : sum;
     }
     PD_RANGE_FN int64_t total() const { return before(groups); }
     // the group that holds the sequence's unit x
@@ -64,8 +78,10 @@ struct TreeSeq {
 };
 
 // From the device's tables as they are (no trust in them: never a negative count). 2^tl tokens per group; causal: no
-// token sees drafted keys after its own.
-PD_RANGE_FN TreeSeq tree_seq(int ip0, int ip1, int last, int q0, int q1, int n_tokens, int tl, int window, int sink, bool causal) {
+// token sees drafted keys after its own. weight: units of a page; of a group that fills at most half of its rows three
+// quarters of that (rounded up). extra: units of a group's start.
+PD_RANGE_FN TreeSeq tree_seq(int ip0, int ip1, int last, int q0, int q1, int n_tokens, int tl, int window, int sink, bool causal,
+                             int weight = 1, int extra = 0) {
     TreeSeq t;
     t.np = ip1 > ip0 ? ip1 - ip0 : 0;
     t.len = t.np > 0 ? (t.np - 1) * 16 + (last < 1 ? 1 : last > 16 ? 16 : last) : 0;
@@ -73,6 +89,9 @@ PD_RANGE_FN TreeSeq tree_seq(int ip0, int ip1, int last, int q0, int q1, int n_t
     t.n = b > a ? b - a : 0;
     t.ctx = t.len - t.n;
     t.groups = (int)(((int64_t)t.n + (1 << tl) - 1) >> tl);
+    t.wt = weight;
+    t.wl = t.n - ((int64_t)(t.groups - 1) << tl) <= (1 << tl) / 2 ? weight - weight / 4 : weight;
+    t.extra = extra;
     t.s = t.w0 = 0;
     if (window > 0) {
         // a token at position ctx or later sees, below the context, only keys from ctx - window + 1 on
@@ -84,7 +103,7 @@ PD_RANGE_FN TreeSeq tree_seq(int ip0, int ip1, int last, int q0, int q1, int n_t
             t.w0 = w0;
         }
     }
-    // A sequence without pages still has its rows to write: one unit an item at least.
+    // A sequence without pages still has its rows to write: one page an item at least.
     t.u0 = t.attended() > 0 ? t.attended() : 1;
     t.st = 0;
     t.cl = 0;
@@ -152,8 +171,7 @@ PD_RANGE_FN TreeCuts tree_cuts(int64_t units, int most, int least, int early, in
     return c;
 }
 
-// The partial slot (0 or 1) of a piece that starts `skip` units into its item and takes `take` of its `units`, or -1: the
-// whole item.
-PD_RANGE_FN int tree_slot(int skip, int take, int units) { return skip > 0 ? 0 : take < units ? 1 : -1; }
+// The partial slot (0 or 1) of a piece that holds pages [p0, p1) of its item's `pages`, or -1: the whole item.
+PD_RANGE_FN int tree_slot(int p0, int p1, int pages) { return p0 > 0 ? 0 : p1 < pages ? 1 : -1; }
 
 }  // namespace pdattn

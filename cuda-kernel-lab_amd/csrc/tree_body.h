@@ -60,8 +60,8 @@ struct TreeScan {
 };
 
 template <class A>
-__device__ __forceinline__ TreeSeq tree_seq_of(const A& a, int ip0, int ip1, int last, int q0, int q1) {
-    return tree_seq(ip0, ip1, last, q0, q1, a.n_tokens, a.tl, a.window, a.sink, a.mask == nullptr);
+__device__ __forceinline__ TreeSeq tree_seq_of(const A& a, int ip0, int ip1, int last, int q0, int q1, int extra) {
+    return tree_seq(ip0, ip1, last, q0, q1, a.n_tokens, a.tl, a.window, a.sink, a.mask == nullptr, a.weight, extra);
 }
 
 // The entries of two sequences in the device's tables in one register, lanes 0 .. 4 and 8 .. 12: the first page-table
@@ -113,7 +113,7 @@ __device__ __forceinline__ int64_t tree_scan_pass(const TreeArgs& a, TreeScan& S
     int64_t mine = 0;
 #pragma unroll
     for (int k = 0; k < kTreeScan; ++k) {
-        f.u[k] = b + k < a.B ? tree_seq_of(a, f.ip[k], f.ip[k + 1], f.last[k], f.q[k], f.q[k + 1]).total() : 0;
+        f.u[k] = b + k < a.B ? tree_seq_of(a, f.ip[k], f.ip[k + 1], f.last[k], f.q[k], f.q[k + 1], a.extra).total() : 0;
         mine += f.u[k];
     }
     int64_t x = mine;
@@ -142,6 +142,7 @@ struct TreeRange {
     int64_t in;       // that unit within sequence b
     int b, left;      // and the units of the range
     int entries;      // of sequences b and b + 1, as tree_load_entry
+    int extra;        // units of an item's start
 };
 template <int NW>
 __device__ __forceinline__ bool tree_find_range(const TreeArgs& a, TreeScan& S, int g, TreeRange& r) {
@@ -156,7 +157,15 @@ __device__ __forceinline__ bool tree_find_range(const TreeArgs& a, TreeScan& S, 
             q0 = q[b];
             q1 = q[b + 1];
         }
-        const int64_t mine = lane < a.B ? tree_seq_of(a, ip0, ip1, last, q0, q1).total() : 0;
+        const TreeSeq seq = tree_seq_of(a, ip0, ip1, last, q0, q1, 0);
+        int64_t mine = lane < a.B ? seq.total() : 0;
+        // Items that are all alike, and a whole number of ranges each: all ranges start one piece, and none has more
+        r.extra = a.extra;
+        const int u = (int)mine;
+        if (a.extra && !__builtin_amdgcn_ballot_w64(lane < a.B && u != __builtin_amdgcn_readfirstlane(u)) &&
+            a.ranges % max(1, a.B * __builtin_amdgcn_readfirstlane(seq.groups)) == 0)
+            r.extra = 0;
+        if (lane < a.B) mine += (int64_t)r.extra * seq.groups;
         if (!__builtin_amdgcn_ballot_w64(mine >> 24 != 0)) {
             int x = (int)mine;   // inclusive sums: within rows of 16 lanes, then from row to row
             x = tree_dpp_add<0x111, 0xF>(x);
@@ -185,6 +194,7 @@ __device__ __forceinline__ bool tree_find_range(const TreeArgs& a, TreeScan& S, 
             return true;
         }
     }
+    r.extra = a.extra;
     constexpr int kPass = kTreeScan * 64 * NW;
     TreeFour f;
     int64_t sum, at = tree_scan_pass<NW>(a, S, 0, f, sum), units = sum;
@@ -1213,9 +1223,9 @@ __device__ __forceinline__ void tree_workgroup(const TreeArgs& a, Sh& S, Piece p
     // the boundary before this range cuts, which of its cuts that is, and its pieces.
     const int lane = threadIdx.x & 63;
     int b = r.b, left = r.left, j, skip;
-    int half = 0, entries = r.entries;   // (the half of the entries that holds sequence b's)
+    int half = 0, entries = lane == 25 ? r.extra : r.entries;   // (half: the entries that hold sequence b's)
     auto entry = [&](int i) { return __builtin_amdgcn_readlane(entries, half + i); };
-    auto sequence = [&](const auto& k) { return tree_seq_of(k, entry(0), entry(1), entry(2), entry(3), entry(4)); };
+    auto sequence = [&](const auto& k) { return tree_seq_of(k, entry(0), entry(1), entry(2), entry(3), entry(4), __builtin_amdgcn_readlane(entries, 25)); };
     {
         const auto& k = *tree_args();
         const TreeSeq t = sequence(k);
@@ -1223,8 +1233,8 @@ __device__ __forceinline__ void tree_workgroup(const TreeArgs& a, Sh& S, Piece p
         skip = __builtin_amdgcn_readfirstlane((int)(r.in - t.before(j)));
         if (kvh == 0 && threadIdx.x == 0) {
             const int64_t first = r.lo - skip;
-            const int g0 = r.cuts.of(first), g1 = r.cuts.of(first + t.units(j) - 1), i0 = j << k.tl;
-            k.cuts[g] = make_int4(max(entry(3), 0) + i0, min(1 << k.tl, t.n - i0) * k.G, skip > 0 ? g1 - g0 + 1 : 0, g - g0 - 1);
+            const int g0 = r.cuts.of(first + t.extra), g1 = r.cuts.of(first + t.last_unit(j)), i0 = j << k.tl;
+            k.cuts[g] = make_int4(max(entry(3), 0) + i0, min(1 << k.tl, t.n - i0) * k.G, g0 < g && g <= g1 ? g1 - g0 + 1 : 0, g - g0 - 1);
         }
     }
     int par = 0;
@@ -1238,26 +1248,30 @@ __device__ __forceinline__ void tree_workgroup(const TreeArgs& a, Sh& S, Piece p
             if (++b >= k.B) break;   // (not reached: the units of the items from here on are at least `left`)
             j = 0;
             const int x = (int)tree_fresh((uint32_t)lane), v = tree_load_entry(k, b + 1, x);
-            entries = (x & 8) == half ? v : entries;
+            entries = (x & 24) == half ? v : entries;
             half ^= 8;
             continue;
         }
-        const int units = p.q.units(j), take = min(left, units - skip);
+        const int take = min(left, p.q.units(j) - skip), f0 = p.q.first_page(j, skip), f1 = p.q.first_page(j, skip + take);
+        left -= take;
+        skip = 0;
+        if (f0 >= f1) {   // no page's first unit: before the item's first or behind its last
+            ++j;
+            continue;
+        }
         p.i0 = j << k.tl;
         p.tokens = min(1 << k.tl, p.q.n - p.i0);
         p.rows = p.tokens * k.G;
-        p.p0 = skip;
-        p.p1 = min(skip + take, p.q.attended());
-        const int s = tree_slot(skip, take, units);
+        p.p0 = f0;
+        p.p1 = min(f1, p.q.attended());
+        const int s = tree_slot(f0, f1, p.q.pages(j));
         p.slot = s < 0 ? -1 : 2 * (int)tree_fresh_s(blockIdx.x) + s;
         p.par = par;
-        left -= take;
-        skip = 0;
         ++j;
         par ^= 1;
         // (the loop's own state is kept in lanes of the entries' register meanwhile)
         const uint32_t x = tree_fresh((uint32_t)lane);
-        entries = x < 16 ? entries : x == 16 ? left : x == 17 ? b : x == 18 ? j : x == 19 ? half | par
+        entries = x < 16 || x > 24 ? entries : x == 16 ? left : x == 17 ? b : x == 18 ? j : x == 19 ? half | par
                 : x == 20 ? p.i0 : x == 21 ? p.rows : x == 22 ? p.q0 : x == 23 ? p.slot : (int)((int)tree_fresh_s(blockIdx.x) * 2 >= k.ranges * k.Hkv);
         entries = (int)tree_fresh((uint32_t)entries);
         piece(p, kvh, entries);

@@ -27,6 +27,12 @@ extern "C" long long t_start(long long units, int most, int least, int early, in
 extern "C" int t_of(long long units, int most, int least, int early, int late, long long x) {
     return tree_cuts(units, most, least, early, late).of(x);
 }
+// the same with `weight` units a page and `extra` an item; a as above
+extern "C" void t_weighted(const int* a, int weight, int extra, int j, int x, int* out) {
+    const TreeSeq t = tree_seq(a[0], a[1], a[2], a[3], a[4], a[5], __builtin_ctz(a[6]), a[7], a[8], a[9] != 0, weight, extra);
+    const long long v[] = {t.units(j), t.before(j), t.total(), t.group_of(t.before(j) + x), t.first_page(j, x), t.groups, t.last_unit(j)};
+    for (int i = 0; i < 7; ++i) out[i] = (int)v[i];
+}
 extern "C" int t_slot(int skip, int take, int units) { return tree_slot(skip, take, units); }
 // out: blocks, the plain ones among them; order[i]: the i-th block
 extern "C" void t_order(int first, int step, int width, int p1, int a0, int a1, int* out, int* order) {

@@ -170,3 +170,76 @@ def test_units_of_a_long_chain(arith, tpg):
     assert [arith.t_before(args, j) for j in range(groups + 1)] == np.concatenate([[0], np.cumsum(units)]).tolist()
     for x in range(0, sum(units), 7):
         assert arith.t_group(args, x) == int(np.searchsorted(np.cumsum(units), x, side="right"))
+
+
+@pytest.mark.parametrize("seed", range(30))
+@pytest.mark.parametrize("weight,extra", [(4, 0), (4, 32), (4, 3), (1, 8)])
+def test_weighted_units(arith, seed, weight, extra):
+    """A last group of at most half its rows counts three quarters, an item's start `extra`; cuts at any unit leave every page
+    in exactly one piece, that of its first unit."""
+    rng = np.random.default_rng(seed)
+    n, tpg, causal = int(rng.integers(1, 300)), int(rng.choice([1, 2, 16, 32, 128])), int(rng.integers(0, 2))
+    length = n + int(rng.choice([0, 3, 100, 4000]))
+    np_ = -(-length // 16)
+    args, out = _args(2, 2 + np_, (length - 1) % 16 + 1, 0, n, n, tpg, 0, 0, causal), (ctypes.c_int * 7)()
+
+    def at(j, x=0):
+        arith.t_weighted(args, weight, extra, j, x, out)
+        return list(out)
+
+    groups, start = -(-n // tpg), 0
+    for j in range(groups):
+        u, before, total, _, _, g, last = at(j)
+        short = 2 * min(tpg, n - j * tpg) <= tpg
+        pages, w = arith.t_units(args, j), weight - weight // 4 if short else weight
+        assert g == groups and before == start and u == pages * w + extra and last == extra + (pages - 1) * w
+        for x in (0, u // 2, u - 1):
+            assert at(j, x)[3] == j
+        cuts = sorted({0, u, *rng.integers(0, u + 1, 5).tolist()})
+        edges = [at(j, c)[4] for c in cuts]
+        assert edges[0] == 0 and edges[-1] == pages and edges == sorted(edges)
+        for c, e in zip(cuts, edges):   # page e is the first whose first unit is c or later
+            assert e == sum(extra + w * k < c for k in range(pages))
+        start += u
+    assert at(0)[2] == start
+
+
+@pytest.mark.parametrize("seed", range(40))
+def test_weighted_pieces_and_their_merges(arith, seed):
+    """The walk of the ranges with starts that count: an item's pieces are whole, in slots of their own, and the merge's
+    arithmetic finds exactly them."""
+    rng = np.random.default_rng(seed)
+    items = [(int(w), int(p)) for w, p in zip(rng.choice([3, 4], 40), rng.integers(1, rng.choice([3, 40, 900]), 40))]
+    extra = int(rng.choice([0, 3, 32, 64]))
+    size = [extra + w * p for w, p in items]
+    firsts = np.concatenate([[0], np.cumsum(size)])
+    cut = (int(firsts[-1]), int(rng.choice([1, 2, 7, 64, 500])), 32, *[(1, 1), (9, 8)][int(rng.integers(0, 2))])
+    R = arith.t_ranges(*cut)
+    starts = [arith.t_start(*cut, g) for g in range(R + 1)]
+    page = lambda k, x: min(max(0, -(-(x - extra) // items[k][0])), items[k][1])  # noqa: E731
+    slots, cover, merges = {}, {k: [] for k in range(len(items))}, {}
+    for g in range(R):
+        k = int(np.searchsorted(firsts, starts[g], side="right")) - 1
+        skip, left = int(starts[g] - firsts[k]), starts[g + 1] - starts[g]
+        w, p = items[k]
+        g0, g1 = arith.t_of(*cut, int(firsts[k]) + extra), arith.t_of(*cut, int(firsts[k]) + extra + w * (p - 1))
+        if g0 < g <= g1:
+            mine = [(g0 + i, 1 if i == 0 else 0) for i in range(g1 - g0 + 1)]
+            assert merges.setdefault(k, mine) == mine
+        while left > 0:
+            take = min(left, size[k] - skip)
+            f0, f1 = page(k, skip), page(k, skip + take)
+            if f0 < f1:
+                s = arith.t_slot(f0, f1, items[k][1])
+                cover[k].append((f0, f1))
+                if s >= 0:
+                    assert (g, s) not in slots, "two pieces in one slot"
+                    slots[g, s] = k
+            left, skip, k = left - take, 0, k + 1
+    for k, (_, p) in enumerate(items):
+        c = cover[k]
+        assert c[0][0] == 0 and c[-1][1] == p and all(a[1] == b[0] for a, b in zip(c, c[1:]))
+        if len(c) > 1:
+            assert [slots[x] for x in merges[k]] == [k] * len(c)
+        else:
+            assert k not in merges
