@@ -57,6 +57,12 @@ size_t align_up(size_t x) { return (x + kAlign - 1) / kAlign * kAlign; }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// n bytes at a and m at b share one
+bool overlap(const void* a, int64_t n, const void* b, int64_t m) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return x < y + (uintptr_t)m && y < x + (uintptr_t)n;
+}
+
 bool valid_group(int G) { return G == 1 || G == 2 || G == 4 || G == 8; }
 
 // Per-device facts cached on first use: CU count, arch name, kernel occupancies.
@@ -1579,6 +1585,14 @@ int pdattn_rope_append_kv(const pdattn_rope_append_params* p, void* stream) {
         if (p->q && p->q_out == p->q && p->q_stride != qw)
             return fail(PDATTN_ERR_INVALID_ARGUMENT, "q_out is contiguous: q can be rotated in place only if it is");
     }
+    if (p->q) {
+        const int64_t out = (int64_t)p->n * p->Hq * kHeadDim * 2;
+        auto meets = [&](const void* x, int64_t stride, int heads) {
+            return overlap(p->q_out, out, x, ((int64_t)(p->n - 1) * stride + (int64_t)heads * kHeadDim) * 2);
+        };
+        if ((p->q_out != p->q && meets(p->q, p->q_stride, p->Hq)) || meets(p->k_new, p->k_stride, p->Hkv) || meets(p->v_new, p->v_stride, p->Hkv))
+            return fail(PDATTN_ERR_INVALID_ARGUMENT, "q_out overlaps an input other than in place");
+    }
     DeviceFacts f;
     if (int st = device_facts(&f)) return st;
     RopeArgs a;
@@ -1685,6 +1699,9 @@ int pdattn_tree_attention(const pdattn_tree_params* p, void* out, float* lse, pd
     if (p->B == 0 || p->n_tokens == 0) return PDATTN_OK;
     if (!out || !lse) return fail(PDATTN_ERR_INVALID_ARGUMENT, "null out / lse");
     if (!aligned16(out)) return fail(PDATTN_ERR_INVALID_ARGUMENT, "out must be 16-byte aligned");
+    // (another workgroup may read a row of q after the first has written it)
+    const int64_t bytes = (int64_t)p->n_tokens * p->Hq * kHeadDim * 2;
+    if (overlap(p->q, bytes, out, bytes)) return fail(PDATTN_ERR_INVALID_ARGUMENT, "out overlaps q");
     TreeLayout L;
     if (int st = tree_layout(p, G, &L)) return st;
     if (int st = ensure_ws(ws, L.bytes)) return st;
@@ -1712,7 +1729,7 @@ int pdattn_tree_attention(const pdattn_tree_params* p, void* out, float* lse, pd
     a.part_lse = reinterpret_cast<float*>(base + L.off_plse);
     a.part_o = reinterpret_cast<float*>(base + L.off_po);
     a.n_tokens = p->n_tokens;
-    a.max_tokens = p->q_indptr ? p->max_tokens : 1;
+    a.max_tokens = p->q_indptr ? std::min(p->max_tokens, p->n_tokens) : 1;   // (its rows fit an int)
     a.mask_words = p->mask_words;
     a.rows = L.rows;
     a.tl = __builtin_ctz((unsigned)(L.rows / G));   // (both powers of two)

@@ -391,7 +391,8 @@ int pdattn_rope_frequencies(int rotary_dim, double base, int scaling, double fac
  * copied. q_out is written for every token, one that is not appended included.
  * q, k_new and v_new are [n, heads, 128] fp16 with *_stride elements from token to token (the heads of
  * a token contiguous), so the three may be slices of one projection's output. q_out [n, Hq, 128] is
- * contiguous and may be q itself (then q_stride = Hq * 128); it may not overlap q otherwise. q = NULL
+ * contiguous and may be q itself (then q_stride = Hq * 128); it may not overlap q otherwise, nor k_new
+ * or v_new (from their first to their last byte). q = NULL
  * (with Hq = 0): only k and v. Pointers and strides are multiples of 16 bytes. */
 typedef struct pdattn_rope_append_params {
     const void*    q;
@@ -462,8 +463,8 @@ typedef struct pdattn_tree_params {
 /* Workspace bytes pdattn_tree_attention needs for `p` (0 on an invalid `p`). They depend on the device
  * and on B, Hq, Hkv, n_tokens, max_tokens and whether q_indptr is NULL alone. */
 size_t pdattn_tree_workspace_size(const pdattn_tree_params* p);
-/* out [n_tokens, Hq, 128] fp16 and lse [n_tokens, Hq] fp32; the workspace as in
- * pdattn_decode_attention. */
+/* out [n_tokens, Hq, 128] fp16, which may not overlap q, and lse [n_tokens, Hq] fp32; the workspace as
+ * in pdattn_decode_attention. */
 int pdattn_tree_attention(const pdattn_tree_params* p, void* out, float* lse, pdattn_workspace* ws,
                           void* stream);
 

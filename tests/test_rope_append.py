@@ -124,6 +124,14 @@ def test_refusals(kw):
     assert e.value.status == 1
 
 
+@pytest.mark.parametrize("kw", [dict(q=(1 << 24) + 2048), dict(q=(1 << 24) - 16), dict(k_new=(1 << 24) + 8176), dict(v_new=(1 << 24) - 512),
+                                dict(q_stride=1 << 22), dict(q=1 << 24, v_new=(1 << 24) + 4096)])
+def test_outputs_over_inputs_are_refused(kw):
+    with pytest.raises(pdattn.PdattnError) as e:
+        pdattn.rope_append_kv(_fake(**kw))
+    assert e.value.status == 1 and "overlaps" in str(e.value)
+
+
 def test_no_tokens():
     pdattn.rope_append_kv(_fake(n=0))
 

@@ -119,6 +119,13 @@ def test_refused_outputs(out, lse):
     assert e.value.status == 1
 
 
+@pytest.mark.parametrize("off", [0, 4 * 8 * 256 - 16, 16 - 4 * 8 * 256])
+def test_an_output_over_the_queries_is_refused(off):
+    with pytest.raises(pdattn.PdattnError) as e:
+        pdattn.tree_attention(_fake(q=1 << 24), (1 << 24) + off, 1 << 20, pdattn.Workspace(1 << 20, 1 << 40, 0))
+    assert e.value.status == 1 and "overlaps" in str(e.value)
+
+
 def test_nothing_to_do():
     ws = pdattn.Workspace()
     pdattn.tree_attention(_fake(B=0, n_tokens=0), 1 << 20, 1 << 20, ws)
@@ -389,6 +396,12 @@ def test_max_tokens_is_a_hint():
         print(f"tree max_tokens {most}", flush=True)
         out, lse = DeviceDraft(dr).run(max_tokens=most)
         check_attention(out, lse, ref, f"max_tokens {most}")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("most", [1, 2 ** 28, 2 ** 29 + 1, 2 ** 31 - 1])
+def test_any_max_tokens_of_a_chain(most):
+    _run(make_draft([300, 20, 77], [5, 30, 1], 8, 2, seed=85, tree=False), f"max_tokens {most}", max_tokens=most)
 
 
 @pytest.mark.gpu
