@@ -1662,10 +1662,13 @@ int tree_layout(const pdattn_tree_params* p, int G, TreeLayout* L) {
     DeviceFacts f;
     if (int st = device_facts(&f)) return st;
     const int64_t rows = (int64_t)(p->q_indptr ? p->max_tokens : 1) * G;
-    // Rows of a workgroup: as many as the longest sequence has, in powers of two. 256 (one workgroup of eight waves a CU)
-    // only where the average is past 128: 8 x 8192 tokens with 256 rows each 96.3 us against 97.7 with 128, 2 x 8192 with
-    // 2048 rows 155.7 against 162.0; but ragged contexts with 40-216 rows, 117 on average, 99 against 83. And only with
-    // plain scores: with changed ones the eight waves' kernel does not fit its registers.
+    // Rows of a workgroup: as many as the longest sequence has, in powers of two. us on 8 x 8192 tokens / on 32 x 200-6000, G = 4:
+    //   up to 32 rows   32: 59.8 / 45.3   64: 59.5 / 47.0
+    //   up to 64        32: 101 / 81.3    64: 61.2 / 55.2    128: 59.2 / 55.8
+    //   up to 128                         64: 83.6 / 94.8    128: 76.5 / 68.8    256: 97.0 / 92.5
+    //   up to 256                         64: 151 / 158      128: 116 / 119      256: 98.8 / 109
+    // 256 (one workgroup of eight waves a CU) only where the average is past 128, as there: 40-216 rows, 117 on average, took
+    // 99 against 83. And only with plain scores: with changed ones the eight waves' kernel does not fit its registers.
     const bool plain = !(p->score.soft_cap > 0.f) && !p->score.slopes && p->score.window <= 0;
     const bool many = plain && rows > 128 && (int64_t)p->n_tokens * G > (int64_t)128 * p->B;
     L->rows = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : many ? 256 : 128;
