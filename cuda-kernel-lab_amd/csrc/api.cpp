@@ -1569,8 +1569,8 @@ int pdattn_rope_append_kv(const pdattn_rope_append_params* p, void* stream) {
     if (p->rotary_dim < 2 || p->rotary_dim > kHeadDim || p->rotary_dim % 2)
         return fail(PDATTN_ERR_INVALID_ARGUMENT, "rotary_dim=%d must be even, in [2, %d]", p->rotary_dim, kHeadDim);
     if (!std::isfinite(p->scale)) return fail(PDATTN_ERR_INVALID_ARGUMENT, "scale is not finite");
+    if (p->n == 0) return PDATTN_OK;   // (an empty tensor's address is NULL)
     if ((p->q == nullptr) != (p->Hq == 0)) return fail(PDATTN_ERR_INVALID_ARGUMENT, "q is NULL just when Hq is 0");
-    if (p->n == 0) return PDATTN_OK;
     if (!p->k_new || !p->v_new || !p->k_cache || !p->v_cache || !p->kv_indptr || !p->kv_indices || !p->batch_idx ||
         !p->positions || !p->freq || (p->q && !p->q_out))
         return fail(PDATTN_ERR_INVALID_ARGUMENT, "null device pointer");
@@ -1744,6 +1744,8 @@ int pdattn_tree_attention(const pdattn_tree_params* p, void* out, float* lse, pd
     a.weight = L.rows == 128 ? 4 : 1;
     a.extra = a.weight * (L.rows <= 32 ? 16 : 8);
     a.least_units = a.weight * 8;
+    // (64 sequences in windows of 1024: 58.3 us with equal ranges, 55.6 with 9 : 8, 56.0 with 17 : 16, 56.3 with 7 : 6; more rows: their
+    // groups, cut at the same keys, share an L2, and 17 : 16 took 66.2 where equal ones took 63.8)
     a.early = L.rows <= 32 ? 9 : 1;
     a.late = L.rows <= 32 ? 8 : 1;
     a.window = std::min(p->score.window, 1 << 30);   // (past any position: sums of positions fit an int)

@@ -174,6 +174,8 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
         raise ValueError("slopes must be contiguous float32 [Hq]")
     _check_tables(q.device, kv_indptr=(kv_indptr, B + 1), kv_indices=(kv_indices, None), kv_last_page_len=(kv_last_page_len, B),
                   q_indptr=(q_indptr, B + 1), mask=(mask, None), depth=(depth, n))
+    if kv_indices.numel() == 0 or k_cache.numel() == 0:   # no key anywhere
+        return torch.zeros_like(q, memory_format=torch.contiguous_format), q.new_full((n, Hq), float("-inf"), dtype=torch.float32)
     q = q.contiguous()
     p = make_tree_params(q, k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len, B, Hq, Hkv, q_indptr=q_indptr,
                          max_tokens=max_tokens, mask=mask, depth=depth, sm_scale=sm_scale, soft_cap=soft_cap, slopes=slopes,
@@ -203,6 +205,8 @@ def accept_kv(k_cache: torch.Tensor, v_cache: torch.Tensor, kv_indptr: torch.Ten
     _check_tables(k_cache.device, kv_indptr=(kv_indptr, B + 1), kv_indices=(kv_indices, None),
                   kv_last_page_len=(kv_last_page_len, B), q_indptr=(q_indptr, B + 1), accepted_indptr=(accepted_indptr, B + 1),
                   accepted=(accepted, None))
+    if accepted.numel() == 0 or kv_indices.numel() == 0:   # nothing to move
+        return
     with torch.cuda.device(k_cache.device):
         _accept_kv(k_cache, v_cache, kv_indptr, kv_indices, kv_last_page_len, q_indptr, accepted_indptr, accepted, B,
                    k_cache.shape[2], stream=torch.cuda.current_stream(k_cache.device))

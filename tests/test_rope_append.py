@@ -134,6 +134,7 @@ def test_outputs_over_inputs_are_refused(kw):
 
 def test_no_tokens():
     pdattn.rope_append_kv(_fake(n=0))
+    pdattn.rope_append_kv(_fake(n=0, q=None, k_new=None, v_new=None, q_out=None))   # as empty tensors give
 
 
 # ---- GPU ----------------------------------------------------------------------------------------------

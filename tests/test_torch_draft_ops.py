@@ -117,3 +117,20 @@ def test_a_traced_step_on_a_side_stream():
     pdattn.workspace_release(ws)
     assert torch.equal(out, d_out) and torch.equal(lse, d_lse)
     assert torch.equal(x["k_cache"], d["k_cache"]) and torch.equal(x["v_cache"], d["v_cache"])
+
+
+@pytest.mark.gpu
+def test_nothing_to_do():
+    """No tokens, no sequences, no pages, nothing accepted."""
+    dev = "cuda:0"
+    i = lambda *v: torch.tensor(v, dtype=torch.int32, device=dev)  # noqa: E731
+    h = lambda *shape: torch.ones(shape, dtype=torch.float16, device=dev)  # noqa: E731
+    ops, kc, vc = torch.ops.pdattn, h(2, 16, 2, 128), h(2, 16, 2, 128)
+    out, lse = ops.tree_attention(h(0, 8, 128), kc, vc, i(0), i(), i(), SCALE, q_indptr=i(0))
+    assert out.shape == (0, 8, 128) and lse.shape == (0, 8)
+    out, lse = ops.tree_attention(h(3, 8, 128), kc, vc, i(0, 0), i(), i(0), SCALE, q_indptr=i(0, 3), max_tokens=3)
+    assert (out == 0).all() and torch.isneginf(lse).all()
+    freq = torch.from_numpy(pdattn.rope_frequencies(64)[0]).to(dev)
+    assert ops.rope_append_kv(h(0, 8, 128), h(0, 2, 128), h(0, 2, 128), kc, vc, i(0, 1), i(1), i(), i(), freq).shape == (0, 8, 128)
+    ops.accept_kv(kc, vc, i(0, 1), i(1), i(3), i(0, 2), i(0, 0), i())
+    assert (kc == 1).all() and (vc == 1).all()
