@@ -238,10 +238,12 @@ def _check(status: int, where: str):
 
 def ptr(x) -> int | None:
     """Device address of x: an int, None, or an object with data_ptr()."""
+    if x is None:
+        return None
     try:
         p = x.data_ptr()
     except AttributeError:
-        if x is None or isinstance(x, int):
+        if isinstance(x, int):
             return x
         raise
     return p if p.__class__ is int else int(p)

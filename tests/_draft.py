@@ -6,7 +6,9 @@ step of fp16 and fp32 relative to the value):
     u16 sum p |v|              the weights' rounding to fp16 in the PV product
     2 u (sum p e |v| + |o| sum p e)   the scores' errors e (oracle.tree_attention's slack), which move a weight p by p e u and
                                through the sum every other; twice for the maximum's part of the exponent
-    (keys / 16 + 64) u sum p |v|, and the same of |o|   sums over the keys: a lane holds at most a sixteenth of them
+    (keys / 16 + 64) u sum p |v|, and the same of |o|   sums over the keys: a lane holds a sixteenth of them where
+                               waves split the keys; where they do not it holds a quarter, held to the same bound (the
+                               roundings of a sum go either way)
 and of lse: 2 u sum p e + (keys / 16 + 64) u + 4 u |lse|. Both twice, for products of these and second orders.
 """
 from dataclasses import dataclass
