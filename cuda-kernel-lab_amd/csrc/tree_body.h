@@ -1318,8 +1318,9 @@ struct TreeMerged {
         const float inv = w == 0.f ? 0.f : 1.f / w;
         const int i = r / a.G;
         const size_t row = (size_t)(cut.x + i) * a.Hq + kvh * a.G + (r - i * a.G);
-        *reinterpret_cast<pf16x4*>(a.out + row * kHeadDim + 4 * c) =
-            pf16x4{(_Float16)(o[0] * inv), (_Float16)(o[1] * inv), (_Float16)(o[2] * inv), (_Float16)(o[3] * inv)};
+        // (not through the L2, which is written back at the kernel's end: chain of 512 on 2 x 8192 150.3 -> 149.4 us)
+        __builtin_nontemporal_store(pf16x4{(_Float16)(o[0] * inv), (_Float16)(o[1] * inv), (_Float16)(o[2] * inv), (_Float16)(o[3] * inv)},
+                                    reinterpret_cast<pf16x4*>(a.out + row * kHeadDim + 4 * c));
         if (c == 0) a.lse[row] = w == 0.f ? -INFINITY : fmaf(__builtin_amdgcn_logf(w), kTreeLn2, m == -INFINITY ? 0.f : m);
     }
 };
